@@ -261,10 +261,7 @@ def _prepare_sampling(case, seed):
 
 def _run_sampling(s):
     if own:
-        if "workspace" not in s:
-            s["workspace"] = _ops().sample_workspace(*s["logits"].shape, s["logits"].device)
-        return _ops().sample_logits(s["logits"], s["uniform"], s["temperature"], s["top_k"], s["top_p"], s["min_p"],
-                                    workspace=s["workspace"])
+        return _ops().sample_logits(s["logits"], s["uniform"], s["temperature"], s["top_k"], s["top_p"], s["min_p"])
     # 64 bits: the cuts and the draw compare sums over the whole vocabulary with a border
     x = s["logits"].double()
     vocab = x.shape[1]
