@@ -485,6 +485,105 @@ NE_API int ne_paged_attention_static_scratch(const void* q, void* out, const voi
                                              const ne_rows* rows, int num_heads, int num_kv_heads, int block_size,
                                              long long num_cache_slots, int splits, int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------- many samples of one prompt */
+/*
+ * Paged attention for a batch whose sequences share prompt prefixes, each prefix's keys and values
+ * read once for all of its sequences (ne_paged_attention reads them once per sequence): a group's
+ * query vectors run together against the prefix, every entry against its own tokens, and the two
+ * parts are merged by their softmax sums. The result is ne_paged_attention's (the reference's
+ * run_cached_attention, models/attention_context.py:66-109), up to rounding.
+ *
+ * Entry b belongs to group entry_group[b] (-1: none, it is served by itself); the first
+ * prefix_blocks[g] block-table entries of a group's members name the same blocks (the first member's
+ * are read). An entry with a row that does not see its whole prefix (position < 16 prefix_blocks - 1)
+ * is served by itself. Rows of entries with q_len 0, and rows of no entry, are left as they were; a
+ * row with a negative position sees no key and gets zeros. Values at positions that a row does not
+ * see do not reach it, whatever they are.
+ */
+typedef struct {
+  int num_groups;                /* groups (0: no entry has one) */
+  int max_prefix_blocks;         /* host bound on prefix_blocks */
+  const int32_t* entry_group;    /* [num_seqs] device */
+  const int32_t* prefix_blocks;  /* [num_groups] device */
+} ne_prefix_groups;
+
+/*
+ * Arguments as ne_paged_attention's. ``workspace`` (256-byte aligned) holds the partial sums of a
+ * call: at least ne_prefix_attention_workspace_bytes() for the call's bounds (NE_ERR_WORKSPACE
+ * otherwise). Calls that can run at the same time need a workspace each. At most 1024 entries and
+ * 32 query heads per KV head. An id outside the pool is reported (NE_DEV_BAD_SLOT) and its tokens
+ * left out.
+ */
+NE_API size_t ne_prefix_attention_workspace_bytes(int max_rows, int num_seqs, int num_groups, int num_heads,
+                                                  int num_kv_heads, int max_q_len, int max_context);
+NE_API int ne_prefix_attention(const void* q, void* out, const void* k_cache, const void* v_cache, const void* k_scale,
+                               const void* v_scale, int kv_int8, const ne_rows* rows, const ne_prefix_groups* groups,
+                               int num_heads, int num_kv_heads, int block_size, long long num_cache_slots,
+                               void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * One draw per row of logits [rows, vocab] (bf16, or fp32 with ``logits_fp32``; rows ``row_stride``
+ * elements apart) from given random numbers. With w_i = exp((x_i - max x) / temperature), the kept
+ * tokens are the first n of the descending order (equal logits: lowest id first), n the least of
+ * top_k (0 or less, or vocab and more: all), the tokens whose mass before them is below top_p times
+ * the mass of the top_k ones (1 or more: all), and those with w_i >= min_p (0 or less: all), and at
+ * least 1. tokens[r] is the first kept id in ascending order whose prefix mass exceeds uniform[r]
+ * (in [0, 1)) times the kept mass, probs[r] (may be NULL) its share of that mass: the inverse CDF of
+ * the sampled steps above, with the cuts of apply_top_p (engine/sampling.py:21-51). temperature 0:
+ * the argmax (lowest id), probability 1. temperature, top_k, top_p and min_p are [rows] device
+ * arrays or NULL (1, 0, 1 and 0 for every row). NaN and -inf logits are never drawn; a row of only
+ * those gives token -1, probability 0 and NE_DEV_BAD_TOKEN. If a logit is +inf, the mass lies on
+ * those that are. Sums are exact in fixed point: equal inputs give equal tokens. vocab <= 262144.
+ */
+NE_API int ne_sample_logits(const void* logits, int logits_fp32, int rows, int vocab, long long row_stride,
+                            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                            const float* uniform, int32_t* tokens, float* probs, int32_t* status, void* stream);
+
+/*
+ * Copy KV blocks within a pool: block src[i] to block dst[i] in every layer, K and V, for the first
+ * *count (device; NULL: max_pairs) pairs. ``kv`` is the pool [num_layers][2][num_cache_slots]
+ * [num_kv_heads][128] (16-byte aligned; bf16, or int8 with ``scales`` [num_layers][2]
+ * [num_cache_slots][num_kv_heads] bf16). A negative src[i] asks for no copy; an id outside the pool
+ * is reported (NE_DEV_BAD_SLOT) and its pair left out. No block may be the destination of two pairs,
+ * nor of one pair and the source of another: the pairs run in no order.
+ */
+NE_API int ne_kv_copy_blocks(void* kv, void* scales, int kv_int8, int num_layers, int num_kv_heads,
+                             long long num_cache_slots, const int32_t* src, const int32_t* dst, const int32_t* count,
+                             int max_pairs, int32_t* status, void* stream);
+
+/*
+ * Fork a sequence: each slot of dst_slots (at most 1024, holding no blocks) becomes a sequence with
+ * the first ``at`` tokens of src_slot's history (0: all of them) and its settings. Its full cached
+ * blocks are src_slot's, shared (num_shared_blocks: src_slot is freed only after its forks); a
+ * partly filled last block is taken from the FIFO, and copy_src[i] -> copy_dst[i] ([num_dst] device)
+ * name the copy that ne_kv_copy_blocks then makes (copy_src -1: none needed). The last token is left
+ * uncached, as after a step, so the next step continues the fork. seeds ([num_dst] device, may be
+ * NULL): new Philox keys, their streams at 0; else the fork continues src_slot's key and position.
+ * A finished source's fork at all tokens stays finished. A destination that is out of range, the
+ * source, listed twice or still holding blocks is refused (NE_DEV_BAD_SLOT, copy_src -2); ``at``
+ * beyond the history (NE_DEV_HISTORY_FULL) or too few free blocks (NE_DEV_OUT_OF_BLOCKS) refuse all.
+ */
+NE_API int ne_state_fork_slots(const ne_batch_state* state, int src_slot, const int32_t* dst_slots, int num_dst, int at,
+                               const uint64_t* seeds, int32_t* copy_src, int32_t* copy_dst, int32_t* status,
+                               void* stream);
+
+/*
+ * Return each listed slot's blocks past its cached tokens (kept for rejected guesses) to the FIFO
+ * tail in table order. Shared blocks stay.
+ */
+NE_API int ne_state_trim_slots(const ne_batch_state* state, const int32_t* slots, int num_slots, int32_t* status,
+                               void* stream);
+
+/*
+ * Compact the pool: the blocks in use move to ids 0 .. used - 1, every slot's block table follows,
+ * and the FIFO then holds the ids from used up, ascending. Writes map [num_blocks] (each block's new
+ * id, -1 for a free one) and the moves move_src -> move_dst ([num_blocks] each), *move_count of them,
+ * which ne_kv_copy_blocks then makes on the same stream. copy_map (may be NULL): the block_map of
+ * ne_model_set_kv_shadow, which follows its blocks. Between steps only.
+ */
+NE_API int ne_state_compact(const ne_batch_state* state, int32_t* map, int32_t* move_src, int32_t* move_dst,
+                            int32_t* move_count, int32_t* copy_map, int32_t* status, void* stream);
+
 /* RMSNorm rows (models/qwen3.py:39-44): y = bf16(bf16(x * rsqrt(mean(x^2) + eps)) * w). */
 NE_API int ne_rmsnorm(const void* x, const void* w, void* y, int rows, int hidden, float eps, void* stream);
 

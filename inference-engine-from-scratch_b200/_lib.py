@@ -68,6 +68,25 @@ EXPORTS = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
          c_longlong, c_int, c_void_p, c_void_p],
     ),
+    "ne_prefix_attention_workspace_bytes": (c_size_t, [c_int] * 7),
+    "ne_prefix_attention": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+         c_longlong, c_void_p, c_size_t, c_void_p, c_void_p],
+    ),
+    "ne_sample_logits": (
+        c_int,
+        [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p],
+    ),
+    "ne_kv_copy_blocks": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
+    ),
+    "ne_state_fork_slots": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p]),
+    "ne_state_trim_slots": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "ne_state_compact": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ne_rmsnorm": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]),
     "ne_sampling_buffer_bytes": (c_size_t, [c_void_p, c_int]),
     "ne_model_set_sampling_buffer": (c_int, [c_void_p, c_void_p, c_size_t, c_int]),
@@ -177,6 +196,11 @@ class BatchState(ctypes.Structure):
 
 class DraftRows(ctypes.Structure):
     _fields_ = [("logits", c_void_p), ("start", c_void_p), ("stride", c_int), ("rows", c_int), ("stats", c_void_p)]
+
+
+class PrefixGroups(ctypes.Structure):
+    _fields_ = [("num_groups", c_int), ("max_prefix_blocks", c_int), ("entry_group", c_void_p),
+                ("prefix_blocks", c_void_p)]
 
 
 class StepOutputs(ctypes.Structure):

@@ -170,6 +170,7 @@ class B200SpeculativeEngine:
         self._prefixes: dict[int, list] = {}      # holder slot -> [tokens, shared blocks, users, copies]
         self._prefix_of: dict[int, int] = {}      # slot -> holder slot of its shared prefix
         self._shared_count: dict[int, int] = {}   # slot -> blocks it shares with its prefix holder
+        self._fork_of: dict[int, int] = {}        # forked slot -> the slot whose blocks it shares
         self.proposed_total = 0
         self.accepted_total = 0
         self.h2d_bytes = 0  # host->device bytes copied for requests and steps
@@ -289,13 +290,65 @@ class B200SpeculativeEngine:
         """Uniforms the request in ``slot`` has drawn from its Philox stream so far (one device read)."""
         return int(self.state.rng_draws[slot].item())
 
+    def fork(self, slot: int, n: int = 1, *, at: int | None = None, seeds: list[int] | None = None) -> list[int]:
+        """Fork a prefilled sequence ``n`` ways: new slots with its tokens (the first ``at`` of them, if
+        given) and settings, on its cached blocks; only a partly filled last block is copied. The
+        forks' next ``step`` (or ``prefill``, for one token) continues them. ``seeds`` key the forks'
+        Philox streams (default: they go on with the source's, and then sample alike). A source is
+        released with or after its forks."""
+        if self.draft_state is not None:
+            raise ValueError("draft-model drafts serve requests without forks")
+        if self._uncached.get(slot, 1 << 30) > 1 or slot in self.state.free_slots:
+            raise ValueError(f"slot {slot} holds no prefilled sequence")
+        if n < 0 or (at is not None and at < 1):
+            raise ValueError("a fork has at least one token, and there are none or more of them")
+        if n > len(self.state.free_slots):
+            raise RuntimeError("no free sequence slot")
+        slots = [self.state.acquire() for _ in range(n)]
+        try:
+            src, dst = self.state.fork(slot, slots, at or 0, seeds)
+        except Exception:
+            self.state.free_slots = slots + self.state.free_slots  # (they hold nothing)
+            raise
+        self.model.copy_blocks(src, dst)
+        for s in slots:
+            self._uncached[s] = 1
+            self._fork_of[s] = slot
+            if slot in self._prefix_of:  # the prefix's blocks are theirs as well
+                self._prefix_of[s] = self._prefix_of[slot]
+                self._prefixes[self._prefix_of[slot]][2] += 1
+                self._shared_count[s] = self._shared_count[slot]
+        return slots
+
+    def trim(self, slots: list[int]) -> None:
+        """Return the blocks that the sequences keep for rejected guesses to the pool (they are
+        reserved again when a step needs them)."""
+        self.state.trim(slots)
+        if self.draft_state is not None:
+            self.draft_state.trim(slots)
+
+    def compact(self) -> int:
+        """Move every block in use to the low end of the pool, so that the blocks from
+        ``num_blocks - num_free_blocks()`` up are free; returns how many moved. Between steps."""
+        copy_map = self.model.kv_copy_map if self.model.kv_copies is not None else None
+        src, dst, count = self.state.compact(copy_map)
+        self.model.copy_blocks(src, dst, count)
+        if self.draft_state is not None:
+            dsrc, ddst, dcount = self.draft_state.compact()
+            self.draft_model.copy_blocks(dsrc, ddst, dcount)
+        return int(count.item())
+
     def release(self, slots: list[int]) -> None:
+        for s, source in self._fork_of.items():
+            if source in slots and s not in slots:
+                raise RuntimeError(f"slot {source} is released with or after its fork {s}")
         self.state.release(slots)
         if self.draft_state is not None:
             self.draft_state.release(slots)
         for s in slots:
             self._uncached.pop(s, None)
             self._shared_count.pop(s, None)
+            self._fork_of.pop(s, None)
             holder = self._prefix_of.pop(s, None)
             if holder is not None:
                 self._prefixes[holder][2] -= 1
@@ -593,6 +646,38 @@ class B200SpeculativeEngine:
                 inflight = None
         if prefix is not None:
             self.drop_prefix(prefix)
+        return outputs
+
+    def generate_samples(self, prompt: list[int], n: int, max_new_tokens: int, ignore_eos: bool = True, *,
+                         temperature: float = 1.0, top_p: float = 1.0, seeds: list[int] | None = None,
+                         prefill_chunk: int | None = None) -> list[list[int]]:
+        """``n`` completions of one prompt (sample i on ``seeds[i]``, default i), which is prefilled
+        once: the others are forks that share its blocks, each with a first token of its own."""
+        if n < 1 or n > self.max_seqs:
+            raise ValueError(f"between 1 and max_seqs = {self.max_seqs} samples")
+        seeds = list(seeds) if seeds is not None else list(range(n))
+        if len(seeds) != n:
+            raise ValueError("one seed per sample")
+        first = self.add_request(prompt, max_new_tokens, ignore_eos=ignore_eos, temperature=temperature, top_p=top_p,
+                                 seed=seeds[0])
+        slots = [first]
+        try:
+            res = self.prefill([first], chunk=prefill_chunk)
+            outputs, finish = [list(res.tokens[first])], [res.finish[first]]
+            if n > 1:
+                slots += self.fork(first, n - 1, at=len(prompt), seeds=seeds[1:])
+                res = self.prefill(slots[1:])
+                outputs += [list(res.tokens[s]) for s in slots[1:]]
+                finish += [res.finish[s] for s in slots[1:]]
+            while any(f is None for f in finish):
+                running = [i for i in range(n) if finish[i] is None]
+                res = self.step([slots[i] for i in running])
+                for i in running:
+                    outputs[i].extend(res.tokens[slots[i]])
+                    finish[i] = res.finish[slots[i]]
+            self.model.raise_on_device_error()
+        finally:
+            self.release(slots)
         return outputs
 
     def _absorb(self, res: StepResult, running: dict[int, int], outputs: list[list[int]]) -> None:

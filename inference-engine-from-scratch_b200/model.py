@@ -221,6 +221,15 @@ class B200Model:
                 merged.append((start, n))
         self._copy_free = merged
 
+    def copy_blocks(self, src: torch.Tensor, dst: torch.Tensor, count: torch.Tensor | None = None) -> None:
+        """Copy KV block ``src[i]`` to ``dst[i]`` in every layer (``ops.copy_kv_blocks``); ids outside
+        the pool are reported in the model's status word."""
+        pairs = src.numel()
+        _lib.check(self.lib.ne_kv_copy_blocks(
+            self.kv.data_ptr(), _lib.ptr(self.kv_scales), int(self.kv_int8), self.cfg.num_hidden_layers,
+            self.cfg.num_key_value_heads, self.num_slots + 1, src.data_ptr(), dst.data_ptr(), _lib.ptr(count), pairs,
+            self.status_ptr, _lib.stream_handle()), "ne_kv_copy_blocks")
+
     # ------------------------------------------------------------------ views
     def k_cache(self, layer: int) -> torch.Tensor:
         return self.kv[layer, 0]

@@ -170,6 +170,58 @@ class DeviceBatchState:
         if word:
             raise _lib.NativeError(f"device reported: {_lib.describe_device_status(word)} (0x{word:x})")
 
+    def _raise_on(self, status: torch.Tensor) -> None:
+        word = int(status.item())
+        if word:
+            raise _lib.NativeError(f"device reported: {_lib.describe_device_status(word)} (0x{word:x})")
+
+    def fork(self, src_slot: int, dst_slots: list[int], at: int = 0,
+             seeds: list[int] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Make each of ``dst_slots`` a sequence of the first ``at`` tokens (0: all) of ``src_slot``,
+        sharing its full cached blocks (ne_state_fork_slots); ``seeds``: the forks' Philox keys (None:
+        they continue the source's stream). Returns the block copies to make (source and destination
+        ids, for ``B200Model.copy_blocks``) before the forks' next step."""
+        if not 0 <= src_slot < self.max_seqs or not 0 <= at <= self.history_stride:
+            raise ValueError(f"no slot {src_slot}, or no {at} tokens to fork at")
+        if seeds is not None and len(seeds) != len(dst_slots):
+            raise ValueError("one seed per fork")
+        n = len(dst_slots)
+        i32 = dict(dtype=torch.int32, device=self.device)
+        pairs = torch.full((2, max(n, 1)), -1, **i32)
+        if n == 0:
+            return pairs[0, :0], pairs[1, :0]
+        ids = torch.tensor(dst_slots, dtype=torch.int32).to(self.device)
+        keys = None if seeds is None else torch.tensor([seed_as_int64(v) for v in seeds]).to(self.device)
+        status = torch.zeros(1, **i32)
+        _lib.check(self.lib.ne_state_fork_slots(self.ref, src_slot, ids.data_ptr(), n, at, _lib.ptr(keys),
+                                                pairs[0].data_ptr(), pairs[1].data_ptr(), status.data_ptr(),
+                                                _lib.stream_handle()), "ne_state_fork_slots")
+        self._raise_on(status)
+        return pairs[0], pairs[1]
+
+    def trim(self, slots: list[int]) -> None:
+        """Return the slots' blocks past their cached tokens to the FIFO (ne_state_trim_slots)."""
+        if not slots:
+            return
+        ids = torch.tensor(slots, dtype=torch.int32).to(self.device)
+        status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        _lib.check(self.lib.ne_state_trim_slots(self.ref, ids.data_ptr(), len(slots), status.data_ptr(),
+                                                _lib.stream_handle()), "ne_state_trim_slots")
+        self._raise_on(status)
+
+    def compact(self, copy_map: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Move the blocks in use to the lowest ids (ne_state_compact). Returns the block copies to
+        make before the next step: source ids, destination ids and their count (one int32, on the
+        device), for ``B200Model.copy_blocks``. ``copy_map``: the block map of the model's dequantised
+        copies, which then follows the blocks."""
+        lists = torch.empty((3, self.num_blocks), dtype=torch.int32, device=self.device)
+        count = torch.zeros(2, dtype=torch.int32, device=self.device)  # moves | status word
+        _lib.check(self.lib.ne_state_compact(self.ref, lists[0].data_ptr(), lists[1].data_ptr(), lists[2].data_ptr(),
+                                             count.data_ptr(), _lib.ptr(copy_map), count[1:].data_ptr(),
+                                             _lib.stream_handle()), "ne_state_compact")
+        self._raise_on(count[1:])
+        return lists[1], lists[2], count[:1]
+
     # ------------------------------------------------------------------ inspection (host copies)
     def block_table(self, slot: int) -> list[int]:
         n = int(self.num_blocks_used[slot].item())

@@ -1,0 +1,216 @@
+"""Draws with temperature, top-k, top-p and min-p from given random numbers (``ops.sample_logits``)
+against the definition in 64 bits on the host: tokens equal, probabilities within a few roundings."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from tests.conftest import submodule
+
+pytestmark = pytest.mark.gpu
+
+SETTINGS = [(0.0, 0, 1.0, 0.0), (0.6, 20, 0.95, 0.0), (0.7, 20, 0.8, 0.0), (1.0, 50, 1.0, 0.0), (0.8, 0, 0.9, 0.0),
+            (1.0, 0, 1.0, 0.05), (1.2, 200, 0.95, 0.02), (1.0, 0, 1.0, 0.0), (1.5, 0, 0.999, 0.0), (1.0, 1, 1.0, 0.0),
+            (3.0, 5000, 0.7, 0.0), (1.0, 0, 0.0, 0.0), (1.0, 0, 1.0, 1.0), (0.05, 0, 0.5, 0.3), (1.0, 1 << 30, 1.0, -1.0)]
+
+
+@pytest.fixture(scope="module")
+def ops(cuda_device):
+    submodule("build").build()
+    return submodule("ops")
+
+
+def expected(x, temperature, top_k, top_p, min_p, u):
+    """(token, probability) of one row by the definition, in 64 bits."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    vocab, top = len(x), x.max()
+    if top == -np.inf:
+        return -1, 0.0
+    if not temperature > 0:
+        return int(np.argmax(x)), 1.0
+    with np.errstate(invalid="ignore"):
+        w = np.where(x == top, 1.0, np.where(x == -np.inf, 0.0, np.exp((x - top) / temperature)))
+    ranked = np.lexsort((np.arange(vocab), -x))
+    if 0 < top_k < vocab:
+        ranked = ranked[:top_k]
+    mass = np.cumsum(w[ranked])
+    kept = len(ranked)
+    if top_p < 1:
+        kept = min(kept, max(1, int((mass - w[ranked] < top_p * mass[-1]).sum())))
+    if min_p > 0:
+        kept = min(kept, max(1, int((w[ranked] >= min_p).sum())))
+    ids = np.sort(ranked[:kept])
+    p = w[ids]
+    below = np.cumsum(p)
+    at = min(int(np.searchsorted(below, u * below[-1], side="right")), kept - 1)
+    return int(ids[at]), float(p[at] / below[-1])
+
+
+def check(ops, logits, settings, uniform, **kw):
+    dev = logits.device
+    rows = logits.shape[0]
+    columns = [torch.tensor([s[i] for s in settings], dtype=torch.int32 if i == 1 else torch.float32, device=dev)
+               for i in range(4)]
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    tokens, probs = ops.sample_logits(logits, uniform, *columns, status=status, **kw)
+    host, u = logits.float().cpu().numpy(), uniform.cpu().numpy().astype(np.float64)
+    floats = [c.cpu().numpy().astype(np.float64) for c in columns]
+    for r in range(rows):
+        token, p = expected(host[r], floats[0][r], int(columns[1][r]), floats[2][r], floats[3][r], u[r])
+        assert int(tokens[r]) == token, (r, settings[r], float(u[r]))
+        # weights in 64 bits, sums in 2^-45 steps, one rounding to fp32
+        assert abs(float(probs[r]) - p) <= 2.0 ** -23 * p + 1e-9, (r, settings[r])
+    return tokens, probs, int(status.item())
+
+
+def language_logits(rows, vocab, seed, device, dtype):
+    g = torch.Generator(device=device).manual_seed(seed)
+    rank = torch.argsort(torch.rand((rows, vocab), generator=g, device=device), dim=-1).float() + 1
+    slope = torch.rand((rows, 1), generator=g, device=device) * 1.5 + 1
+    x = 15 - slope * torch.log(rank) + torch.randn((rows, vocab), generator=g, device=device)
+    u = torch.randint(0, 1 << 24, (rows,), generator=g, device=device).float() * 2.0 ** -24
+    return x.to(dtype), u
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 31, 100, 1000, 4096, 8192, 8193, 16387, 50021, 151936, 262144])
+def test_matches_the_definition(ops, cuda_device, vocab, dtype) -> None:
+    logits, u = language_logits(len(SETTINGS), vocab, vocab, cuda_device, dtype)
+    _, _, status = check(ops, logits, SETTINGS, u)
+    assert status == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_many_rows(ops, cuda_device, dtype) -> None:
+    rows = 200
+    logits, u = language_logits(rows, 12345, 3, cuda_device, dtype)
+    check(ops, logits, [SETTINGS[r % len(SETTINGS)] for r in range(rows)], u)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [40, 5000, 70001])
+def test_ties_go_to_the_lowest_ids(ops, cuda_device, vocab, dtype) -> None:
+    """A handful of distinct values: every cut falls inside a group of equal logits."""
+    g = torch.Generator().manual_seed(vocab)
+    logits = torch.randint(0, 5, (len(SETTINGS), vocab), generator=g).to(dtype).to(cuda_device)
+    logits[3] = 1.5   # all equal
+    logits[7] = -2.0
+    logits[4] = 0.0
+    logits[4, ::2] = -0.0  # equal to 0
+    u = torch.rand(len(SETTINGS), generator=g).to(cuda_device)
+    check(ops, logits, SETTINGS, u)
+
+
+def test_first_and_last_random_number(ops, cuda_device) -> None:
+    for u in (0.0, 1.0 - 2.0 ** -24):
+        logits, uniform = language_logits(len(SETTINGS), 20000, 9, cuda_device, torch.bfloat16)
+        uniform.fill_(u)
+        check(ops, logits, SETTINGS, uniform)
+    # a number of 1 or more takes the last kept token, one below 0 or NaN the first
+    logits = torch.zeros(3, 10, device=cuda_device)
+    tokens, probs = ops.sample_logits(logits, torch.tensor([1.0, -1.0, float("nan")], device=cuda_device))
+    assert tokens.tolist() == [9, 0, 0]
+    torch.testing.assert_close(probs, torch.full_like(probs, 0.1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_masked_infinite_and_nan_logits(ops, cuda_device, dtype) -> None:
+    n = len(SETTINGS)
+    logits, u = language_logits(n, 9001, 21, cuda_device, dtype)
+    logits[:, ::3] = float("-inf")
+    logits[:, 1::7] = float("nan")
+    logits[:, 5] = torch.finfo(dtype).min
+    _, _, status = check(ops, logits, SETTINGS, u)
+    assert status == 0
+    logits[:, 100] = float("inf")
+    logits[:, 7000] = float("inf")
+    logits[2, 7000] = float("nan")
+    _, _, status = check(ops, logits, SETTINGS, u)
+    assert status == 0
+    only = torch.full_like(logits, float("-inf"))
+    only[:, 4444] = -3.0
+    check(ops, only, SETTINGS, u)
+    only[1] = float("-inf")
+    only[4] = float("nan")
+    tokens, probs, status = check(ops, only, SETTINGS, u)
+    assert status == 8 and tokens[1] == -1 and probs[4] == 0
+
+
+def test_extreme_temperatures(ops, cuda_device) -> None:
+    logits, u = language_logits(6, 3000, 5, cuda_device, torch.float32)
+    settings = [(1e-6, 0, 1.0, 0.0), (1e-6, 0, 0.9, 0.0), (1e4, 0, 0.5, 0.0), (1e4, 700, 0.5, 0.0), (1e30, 0, 1.0, 0.0),
+                (1e30, 0, 0.3, 0.5)]
+    check(ops, logits, settings, u)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_strided_and_misaligned_rows(ops, cuda_device, dtype) -> None:
+    for vocab, width, shift in ((1001, 1003, 0), (1001, 1008, 3), (9000, 9001, 1), (17, 40, 5)):
+        base, u = language_logits(len(SETTINGS), width, vocab, cuda_device, dtype)
+        check(ops, base[:, shift: shift + vocab], SETTINGS, u)
+
+
+def test_no_settings_is_a_plain_draw_and_none_equals_neutral(ops, cuda_device) -> None:
+    logits, u = language_logits(32, 6000, 6, cuda_device, torch.bfloat16)
+    plain, p0 = ops.sample_logits(logits, u)
+    neutral, p1 = ops.sample_logits(logits, u, torch.ones(32, device=cuda_device),
+                                    torch.zeros(32, dtype=torch.int32, device=cuda_device),
+                                    torch.ones(32, device=cuda_device), torch.zeros(32, device=cuda_device))
+    assert torch.equal(plain, neutral) and torch.equal(p0, p1)
+    check(ops, logits, [(1.0, 0, 1.0, 0.0)] * 32, u)
+
+
+def test_equals_the_sampled_steps_draw(ops, cuda_device) -> None:
+    """A draw without guesses in the verify step (temperature and top-p on a Philox stream) takes the
+    same token as this operator with the stream's uniform."""
+    serial = submodule("serial")
+    from oracle.philox import uniform as philox_uniform
+    logits, _ = language_logits(24, 4096, 8, cuda_device, torch.bfloat16)
+
+    class Params:
+        temperature, top_p = 0.9, 0.85
+
+    for r in range(24):
+        gen = serial.PhiloxGenerator(1000 + r)
+        want = serial._logits_verifier(cuda_device).verify([], logits[r: r + 1], Params, gen)
+        u = torch.tensor([float(philox_uniform(1000 + r, 0))], device=cuda_device)
+        got, _ = ops.sample_logits(logits[r: r + 1], u, torch.tensor([0.9], device=cuda_device), None,
+                                   torch.tensor([0.85], device=cuda_device))
+        assert got.tolist() == want
+
+
+def test_capture_and_side_stream(ops, cuda_device) -> None:
+    logits, u = language_logits(len(SETTINGS), 30000, 12, cuda_device, torch.bfloat16)
+    columns = [torch.tensor([s[i] for s in SETTINGS], dtype=torch.int32 if i == 1 else torch.float32,
+                            device=cuda_device) for i in range(4)]
+    want, _ = ops.sample_logits(logits, u, *columns)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, _ = ops.sample_logits(logits, u, *columns)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, _ = ops.sample_logits(logits, u, *columns)
+    other, u2 = language_logits(len(SETTINGS), 30000, 13, cuda_device, torch.bfloat16)
+    logits.copy_(other)
+    u.copy_(u2)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, _ = ops.sample_logits(other, u2, *columns)
+    assert torch.equal(got, want)
+
+
+def test_no_rows_and_refusals(ops, cuda_device) -> None:
+    tokens, probs = ops.sample_logits(torch.zeros(0, 8, device=cuda_device), torch.zeros(0, device=cuda_device))
+    assert tokens.shape == (0,) and probs.shape == (0,)
+    logits, u = torch.zeros(2, 8, device=cuda_device), torch.zeros(2, device=cuda_device)
+    for args in ((logits.half(), u), (logits.t(), u), (logits, u[:1]), (logits, u.double()), (logits[:, ::2], u),
+                 (logits[0], u), (torch.zeros(1, 8, device=cuda_device).expand(2, 8), u), (logits, u, None, u)):
+        with pytest.raises(ValueError):
+            ops.sample_logits(*args)
+    with pytest.raises(submodule("_lib").NativeError):
+        ops.sample_logits(torch.zeros(1, 262145, device=cuda_device), u[:1])
