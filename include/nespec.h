@@ -495,8 +495,9 @@ NE_API int ne_paged_attention_static_scratch(const void* q, void* out, const voi
  *
  * Entry b belongs to group entry_group[b] (-1: none, it is served by itself); the first
  * prefix_blocks[g] block-table entries of a group's members name the same blocks (the first member's
- * are read). An entry with a row that does not see its whole prefix (position < 16 prefix_blocks - 1)
- * is served by itself. Rows of entries with q_len 0, and rows of no entry, are left as they were; a
+ * are read). An entry with a row that does not see its whole prefix (position < 16 prefix_blocks - 1),
+ * or whose prefix is longer than max_prefix_blocks or its table, is served by itself. Entries have
+ * rows of their own, at ascending positions. Rows of entries with q_len 0, and rows of no entry, are left as they were; a
  * row with a negative position sees no key and gets zeros. Values at positions that a row does not
  * see do not reach it, whatever they are.
  */
@@ -510,7 +511,7 @@ typedef struct {
 /*
  * Arguments as ne_paged_attention's. ``workspace`` (256-byte aligned) holds the partial sums of a
  * call: at least ne_prefix_attention_workspace_bytes() for the call's bounds (NE_ERR_WORKSPACE
- * otherwise). Calls that can run at the same time need a workspace each. At most 1024 entries and
+ * otherwise); k_cache and v_cache are 128-byte aligned, q and out 16-byte. Calls that can run at the same time need a workspace each. At most 1024 entries and
  * 32 query heads per KV head. An id outside the pool is reported (NE_DEV_BAD_SLOT) and its tokens
  * left out.
  */

@@ -1,75 +1,1074 @@
 // Paged attention for a batch whose sequences share prompt prefixes (include/nespec.h,
-// ne_prefix_attention): the simplest kernel that is right for every case. A warp serves one query
-// vector against its sequence's whole context, 32 keys at a time: a key per lane for the scores, four
-// dimensions per lane for the values.
+// ne_prefix_attention), in three launches:
+//
+// * own_tokens_kernel: every entry against the tokens that are its own (all of them for an entry
+//   without a group), 16 query vectors a tile on mma.sync, one CTA per (entry, KV head, tile, split).
+// * prefix_kernel: every group's query vectors, gathered over its entries, against its prefix:
+//   tcgen05 tiles of 128 vectors x 128 keys, persistent CTAs that divide all prefixes' tiles evenly.
+// * join_kernel: o = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m) over an entry's parts i, each an
+//   unnormalised sum O_i of values, its sum of weights l_i and the (log2) reference m_i of both.
+#include <algorithm>
+
 #include "attention.cuh"
+#include "attention_tile.cuh"
+#include "gemm_tc.cuh"
 
 namespace ne {
 
 namespace {
 
-constexpr int D = 128;
+constexpr int MAX_SEQS = 1024;   // entries of a launch (the plan of prefix_kernel is in shared memory)
+constexpr int MAX_GROUP = 32;    // query heads per KV head
+constexpr int TILE = 128;        // query vectors, and keys, of a tensor-core tile
 constexpr unsigned ALL = 0xFFFFFFFFu;
 
-__global__ void __launch_bounds__(128)
-    row_attention_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out,
-                         const void* __restrict__ kc, const void* __restrict__ vc, const __nv_bfloat16* __restrict__ ks,
-                         const __nv_bfloat16* __restrict__ vs, int kv_int8, ne_rows rows, int nh, int nkv,
-                         long long num_cache_slots, int* status) {
-  pdl_prologue();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x;
-  const int ql = rows.q_len[b];
-  const int v = blockIdx.y * 4 + warp;  // vector of the entry: row v / nh, head v % nh
-  if (v >= ql * nh) return;
-  const int row = rows.q_start[b] + v / nh, head = v % nh, h = head / (nh / nkv);
-  const int pos = rows.positions[row];
-  const int32_t* table =
-      rows.block_tables + (long long)(rows.table_index ? rows.table_index[b] : b) * rows.block_table_stride;
-  const __nv_bfloat16* qr = q + ((long long)row * nh + head) * D;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 <= pos; k0 += 32) {
-    const int key = k0 + lane;
-    long long slot = -1;
-    if (key <= pos) {
-      const long long blk = key / 16 < rows.block_table_stride ? table[key / 16] : -1;
-      if (blk < 0 || (blk + 1) * 16 > num_cache_slots - 1) report(status, NE_DEV_BAD_SLOT);
-      else slot = blk * 16 + key % 16;
+// ---------------------------------------------------------------- the parts of a call, in its workspace
+struct Parts {
+  // own tokens: [split][row][head]
+  float *own_o, *own_m, *own_l;
+  // prefixes: per part up to 256 vectors at an offset of their own (prefix_offset)
+  float *pre_o, *pre_m, *pre_l;
+  // the plan, written by prefix_kernel's first CTA for the join
+  int32_t* entry_at;      // [num_seqs] the entry's first row among its group's
+  long long* group_work;  // [num_groups + 1] work before group g (its units: see Plan)
+  long long* group_vec;   // [num_groups + 1] vectors of one KV head before group g
+  int splits;
+};
+
+constexpr size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+struct Layout {
+  size_t own_o, own_m, own_l, pre_o, pre_m, pre_l, entry_at, group_work, group_vec, total;
+};
+
+// Vectors of the prefixes' parts: each item's twice (an item of one tile has two parts, one of two
+// tiles a part of each), and 256 more for every boundary between CTAs (see prefix_offset).
+inline long long prefix_part_vectors(long long max_rows, int nh, int ctas) {
+  return 2 * max_rows * nh + 256LL * (ctas + 1);
+}
+
+inline Layout layout_of(long long max_rows, int num_seqs, int num_groups, int nh, int splits, int ctas) {
+  Layout l;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t p = at;
+    at += align256(bytes);
+    return p;
+  };
+  const size_t own = (size_t)splits * max_rows * nh;
+  const size_t pre = num_groups > 0 ? (size_t)prefix_part_vectors(max_rows, nh, ctas) : 0;
+  l.own_o = take(own * D * 4);
+  l.own_m = take(own * 4);
+  l.own_l = take(own * 4);
+  l.pre_o = take(pre * D * 4);
+  l.pre_m = take(pre * 4);
+  l.pre_l = take(pre * 4);
+  l.entry_at = take((size_t)num_seqs * 4);
+  l.group_work = take(((size_t)num_groups + 1) * 8);
+  l.group_vec = take(((size_t)num_groups + 1) * 8);
+  l.total = at;
+  return l;
+}
+
+// ---------------------------------------------------------------- entries and groups
+struct Entry {
+  int rows, start, group;  // rows 0: nothing to do; group -1: no shared prefix
+};
+
+// Entry b as every kernel of the call sees it. Rows outside the host's bounds are reported and left
+// out; a group is taken only if the entry's first row (its positions ascend) sees its whole prefix.
+__device__ __forceinline__ Entry entry_of(const ne_rows& rows, const ne_prefix_groups& groups, int b, int* status) {
+  Entry e{rows.q_len[b], rows.q_start[b], -1};
+  if (e.rows <= 0) return Entry{0, 0, -1};
+  const int g = groups.num_groups > 0 ? groups.entry_group[b] : -1;
+  if (e.rows > rows.max_q_len || e.start < 0 || e.start > rows.max_rows - e.rows) {
+    report(status, NE_DEV_BAD_SLOT);
+    return Entry{0, 0, -1};
+  }
+  const int first = rows.positions[e.start];
+  if (g >= 0 && g < groups.num_groups) {
+    const int blocks = groups.prefix_blocks[g];
+    if (blocks > 0 && blocks <= min(rows.block_table_stride, groups.max_prefix_blocks) && first >= blocks * 16 - 1) e.group = g;
+  }
+  return e;
+}
+
+__device__ __forceinline__ const int32_t* table_of(const ne_rows& rows, int b) {
+  return rows.block_tables + (long long)(rows.table_index ? rows.table_index[b] : b) * rows.block_table_stride;
+}
+
+// ---------------------------------------------------------------- own tokens
+// One 16-token block (logical index kb) against the tile, as tile_block, but values at masked keys do
+// not reach the sums whatever they are, and an int8 block holds its integers as they are: the K scale
+// (``scales``: lane t token t's, lane 16 + t its V scale) multiplies the scores, the V scale the
+// weights, both in fp32 (one rounding of the weights, none of keys and values).
+template <bool INT8>
+__device__ __forceinline__ void own_block(TileState& ts, uint32_t k_s, uint32_t v_s, int kb, uint32_t scales,
+                                          int lane) {
+  float s[2][4];
+  float mx[2] = {NEG_INF, NEG_INF};
+  bool masked = false;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 8; kk += 2) {
+      uint32_t b[4];
+      const int tok = 8 * j + (lane & 7);
+      const int col = 16 * kk + 8 * (lane >> 3);
+      ldsm_x4(b, kv_addr<false>(k_s, tok, col));
+      mma16816(s[j], ts.qa[kk], b[0], b[1]);
+      mma16816(s[j], ts.qa[kk + 1], b[2], b[3]);
     }
-    float s = -INFINITY;
-    if (slot >= 0) {
-      const long long at = (slot * nkv + h) * D;
-      const float scale = kv_int8 ? ld_bf16(ks + slot * nkv + h) : 1.f;
-      float dot = 0.f;
-      for (int d = 0; d < D; ++d)
-        dot += ld_bf16(qr + d) * (kv_int8 ? (float)static_cast<const int8_t*>(kc)[at + d]
-                                          : ld_bf16(static_cast<const __nv_bfloat16*>(kc) + at + d));
-      s = dot * scale * 0.08838834764831845f;  // 1 / sqrt(128)
+    float ks[2] = {SCALE_LOG2, SCALE_LOG2};
+    if (INT8) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        ks[x] *= __uint_as_float(__shfl_sync(ALL, scales, 8 * j + 2 * (lane & 3) + x) << 16);
     }
-    float top = s;
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(ALL, top, x));
-    const float mn = fmaxf(m, top);
-    if (mn == -INFINITY) continue;
-    const float c = expf(m - mn), p = slot >= 0 ? expf(s - mn) : 0.f;
-    m = mn;
-    float sum = p;
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(ALL, sum, x);
-    l = l * c + sum;
-    for (int j = 0; j < 4; ++j) o[j] *= c;
-    for (int t = 0; t < 32; ++t) {
-      const long long st = __shfl_sync(ALL, slot, t);
-      if (st < 0) continue;
-      const float pt = __shfl_sync(ALL, p, t) * (kv_int8 ? ld_bf16(vs + st * nkv + h) : 1.f);
-      const long long at = (st * nkv + h) * D + 4 * lane;
-      for (int j = 0; j < 4; ++j)
-        o[j] += pt * (kv_int8 ? (float)static_cast<const int8_t*>(vc)[at + j]
-                              : ld_bf16(static_cast<const __nv_bfloat16*>(vc) + at + j));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = e >> 1;
+      const int key = kb * 16 + 8 * j + 2 * (lane & 3) + (e & 1);
+      float v = s[j][e] * ks[e & 1];
+      if (key > ts.pos[r]) {
+        v = NEG_INF;
+        masked |= ts.pos[r] >= 0;  // (a row without keys has no sums to keep clean)
+      }
+      s[j][e] = v;
+      mx[r] = fmaxf(mx[r], v);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-  for (int j = 0; j < 4; ++j)
-    out[((long long)row * nh + head) * D + 4 * lane + j] = __float2bfloat16_rn(o[j] * inv);
+  float corr[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    mx[r] = fmaxf(mx[r], __shfl_xor_sync(ALL, mx[r], 1));
+    mx[r] = fmaxf(mx[r], __shfl_xor_sync(ALL, mx[r], 2));
+    const float m_new = fmaxf(ts.m[r], mx[r]);
+    corr[r] = (m_new == NEG_INF || ts.m[r] == NEG_INF) ? (m_new == NEG_INF ? 1.f : 0.f) : exp2f(ts.m[r] - m_new);
+    ts.m[r] = m_new;
+  }
+  float psum[2] = {0.f, 0.f}, p[2][4];
+  uint32_t pa[4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = e >> 1;
+      p[j][e] = (s[j][e] == NEG_INF) ? 0.f : exp2f(s[j][e] - ts.m[r]);
+      psum[r] += p[j][e];
+    }
+    if (INT8) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float vs = __uint_as_float(__shfl_sync(ALL, scales, 16 + 8 * j + 2 * (lane & 3) + (e & 1)) << 16);
+        p[j][e] = (s[j][e] == NEG_INF) ? 0.f : p[j][e] * vs;
+      }
+    }
+    pa[2 * j] = pack_bf16(p[j][0], p[j][1]);
+    pa[2 * j + 1] = pack_bf16(p[j][2], p[j][3]);
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    psum[r] += __shfl_xor_sync(ALL, psum[r], 1);
+    psum[r] += __shfl_xor_sync(ALL, psum[r], 2);
+    ts.l[r] = ts.l[r] * corr[r] + psum[r];
+  }
+  if (__any_sync(ALL, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      ts.o[t][0] *= corr[0];
+      ts.o[t][1] *= corr[0];
+      ts.o[t][2] *= corr[1];
+      ts.o[t][3] *= corr[1];
+    }
+  }
+  // a block with masked keys (the last one or two of an entry): 0 x inf or 0 x NaN must stay out
+  bool plain = true;
+  if (!INT8 && __any_sync(ALL, masked)) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int x = lane + 32 * i;  // 16 tokens x 16 chunks of 8 values
+      uint32_t w[4];
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                   : "r"(kv_addr<false>(v_s, x >> 4, 8 * (x & 15))));
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        odd |= (w[y] & 0x7F80u) == 0x7F80u || (w[y] & 0x7F800000u) == 0x7F800000u;
+    }
+    plain = !__any_sync(ALL, odd);
+  }
+  if (plain) {
+#pragma unroll
+    for (int t = 0; t < 16; t += 2) {
+      uint32_t b[4];
+      const int tok = (lane & 7) + 8 * ((lane >> 3) & 1);
+      const int col = 8 * t + 8 * (lane >> 4);
+      ldsm_x4_t(b, kv_addr<false>(v_s, tok, col));
+      mma16816(ts.o[t], pa, b[0], b[1]);
+      mma16816(ts.o[t + 1], pa, b[2], b[3]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int tok = 0; tok < 16; ++tok) {  // (seldom: some value of the block is infinite or NaN)
+    const int from = (lane & ~3) | ((tok & 7) >> 1);
+    float w[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) w[r] = bf16r(__shfl_sync(ALL, p[tok >> 3][2 * r + (tok & 1)], from));
+    const int key = kb * 16 + tok;
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      uint32_t v;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(kv_addr<false>(v_s, tok, 8 * t) + 4 * (lane & 3)));
+      const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xFFFF0000u);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (key > ts.pos[r]) continue;
+        ts.o[t][2 * r] += w[r] * v0;
+        ts.o[t][2 * r + 1] += w[r] * v1;
+      }
+    }
+  }
 }
+
+constexpr int OWN_WARPS = 4;
+constexpr size_t OWN_SMEM = BLOCK_BYTES + 128 + (size_t)OWN_WARPS * 4 * BLOCK_BYTES;
+static_assert((OWN_WARPS * 16 * D + 2 * OWN_WARPS * 16) * 4 <= OWN_WARPS * 4 * BLOCK_BYTES, "merge area");
+
+// The four warps take every fourth block of the split, each with two cp.async stages of its own, and
+// merge their sums through shared memory. Bound by memory: each block is read once per tile.
+template <bool INT8>
+__global__ void __launch_bounds__(32 * OWN_WARPS, 3)
+    own_tokens_kernel(const __nv_bfloat16* __restrict__ q, const void* __restrict__ kc, const void* __restrict__ vc,
+                      const __nv_bfloat16* __restrict__ ks, const __nv_bfloat16* __restrict__ vs, ne_rows rows,
+                      ne_prefix_groups groups, int nh, int nkv, long long num_cache_slots, Parts parts, int tiles,
+                      int* status) {
+  pdl_prologue();
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int b = blockIdx.x, h = blockIdx.y, tile = blockIdx.z % tiles, split = blockIdx.z / tiles;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Entry e = entry_of(rows, groups, b, tid == 0 && tile == 0 && h == 0 && split == 0 ? status : nullptr);
+  Ctx c{};
+  c.G = nh / nkv;
+  c.nvec = e.rows * c.G;
+  const int v_base = 16 * tile;
+  if (v_base >= c.nvec) return;
+  c.q = q;
+  c.kc = kc;
+  c.vc = vc;
+  c.ks = ks;
+  c.vs = vs;
+  c.table = table_of(rows, b);
+  c.nh = nh;
+  c.nkv = nkv;
+  c.h = h;
+  c.r0 = e.start;
+  c.num_cache_slots = num_cache_slots;
+  c.status = status;
+  uint8_t* q_s = smem;
+  int* spos = reinterpret_cast<int*>(smem + BLOCK_BYTES);
+  uint8_t* buf = smem + BLOCK_BYTES + 128;
+  const uint32_t wbuf = smem_u32(buf) + warp * 4 * BLOCK_BYTES;
+  const int v_last = min(c.nvec, v_base + 16) - 1;
+  const int last = rows.positions[c.r0 + v_last / c.G];  // the tile's last row sees the most
+  const int nblk = last >= 0 ? last / 16 + 1 : 0;
+  const int kb_first = e.group >= 0 ? groups.prefix_blocks[e.group] : 0;
+  const int n = max(0, nblk - kb_first), per_split = (n + parts.splits - 1) / parts.splits;
+  const int kb0 = kb_first + split * per_split, kb1 = min(nblk, kb0 + per_split);
+  const int stride = rows.block_table_stride;
+  // this warp's blocks kb0 + warp + 4 j; the table entries of 32 of them in the lanes of a register
+  const int count = kb0 + warp < kb1 ? (kb1 - kb0 - warp + OWN_WARPS - 1) / OWN_WARPS : 0;
+  auto table_chunk = [&](int j0) -> int {
+    const int kb = kb0 + warp + OWN_WARPS * (j0 + lane);
+    return kb < kb1 && kb < stride ? c.table[kb] : -1;
+  };
+  int tbl = table_chunk(0);
+  auto block_at = [&](int j) -> long long {  // (warp-uniform; an id that names no block is reported)
+    if ((j & 31) == 0 && j > 0) tbl = table_chunk(j);
+    return checked_block(c, __shfl_sync(ALL, tbl, j & 31));
+  };
+  uint32_t scales = 0, next_scales = 0;
+  auto stage = [&](int j, long long blk) {
+    if (blk >= 0) {
+      if (INT8) {
+        stage_raw_int8(c, blk, wbuf + (j & 1) * 4096, lane);
+        next_scales = load_scales_int8(c, blk, lane);
+      } else {
+        const uint32_t at = wbuf + (j & 1) * 2 * BLOCK_BYTES;
+        stage_block<false>(c, blk, at, at + BLOCK_BYTES, lane, 32);
+      }
+    }
+    cp_commit();
+  };
+  long long blk = count > 0 ? block_at(0) : -1;
+  stage(0, blk);
+  if (tid < 16) spos[tid] = v_base + tid < c.nvec ? rows.positions[c.r0 + (v_base + tid) / c.G] : -1;
+  load_q_tile(c, v_base, q_s, tid, 32 * OWN_WARPS);
+  __syncthreads();
+  TileState ts;
+  tile_init(ts, smem_u32(q_s), spos, lane);
+  for (int j = 0; j < count; ++j) {
+    scales = next_scales;
+    const long long next = j + 1 < count ? block_at(j + 1) : -1;
+    stage(j + 1, next);
+    cp_wait<1>();
+    __syncwarp();
+    if (blk >= 0) {
+      const int kb = kb0 + warp + OWN_WARPS * j;
+      if (INT8) {
+        const uint32_t raw = wbuf + (j & 1) * 4096, kv = wbuf + 8192;
+        convert_raw_int8(raw, kv, kv + BLOCK_BYTES, 0x3F80u, lane);  // (scale 1: the integers, exact in bf16)
+        __syncwarp();
+        own_block<true>(ts, kv, kv + BLOCK_BYTES, kb, scales, lane);
+      } else {
+        const uint32_t at = wbuf + (j & 1) * 2 * BLOCK_BYTES;
+        own_block<false>(ts, at, at + BLOCK_BYTES, kb, 0u, lane);
+      }
+    }
+    __syncwarp();
+    blk = next;
+  }
+  cp_wait<0>();
+  __syncthreads();
+  float* mo = reinterpret_cast<float*>(buf);  // [warps][16][128]
+  float* mm = mo + OWN_WARPS * 16 * D;        // [warps][16]
+  float* ml = mm + OWN_WARPS * 16;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = (lane >> 2) + 8 * r;
+#pragma unroll
+    for (int t = 0; t < 16; ++t)
+      *reinterpret_cast<float2*>(&mo[(warp * 16 + row) * D + 8 * t + 2 * (lane & 3)]) =
+          make_float2(ts.o[t][2 * r], ts.o[t][2 * r + 1]);
+    if ((lane & 3) == 0) {
+      mm[warp * 16 + row] = ts.m[r];
+      ml[warp * 16 + row] = ts.l[r];
+    }
+  }
+  __syncthreads();
+  for (int v = 0; v < v_last - v_base + 1; ++v) {
+    float m = NEG_INF, l = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < OWN_WARPS; ++w) m = fmaxf(m, mm[w * 16 + v]);
+#pragma unroll
+    for (int w = 0; w < OWN_WARPS; ++w) {
+      const float mw = mm[w * 16 + v];
+      const float f = mw == NEG_INF ? 0.f : exp2f(mw - m);
+      if (f != 0.f) {
+        l += ml[w * 16 + v] * f;
+        o += mo[(w * 16 + v) * D + tid] * f;
+      }
+    }
+    const int row = c.r0 + (v_base + v) / c.G, head = h * c.G + (v_base + v) % c.G;
+    const long long at = ((long long)split * rows.max_rows + row) * nh + head;
+    parts.own_o[at * D + tid] = o;
+    if (tid == 0) {
+      parts.own_m[at] = m;
+      parts.own_l[at] = l;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- prefixes: the division of the work
+// A group's vectors of one KV head are cut into items of up to 256. An item of more than 128 is two
+// query tiles that share every tile of 128 keys (2 units of work a key tile); a smaller one is one
+// query tile whose two halves of the SM take every second key tile (1 unit). The units of all (group,
+// head, item) in turn are divided evenly over the CTAs: CTA c does the key tiles that start in units
+// [c W / n, (c + 1) W / n).
+struct Group {
+  int vec, blocks;        // query vectors of one KV head, prefix blocks
+  long long work, vec_at;  // units before it; vectors (of one KV head) before it
+};
+__device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 7) / 8; }
+__device__ __forceinline__ int item_units(int vec) { return vec > TILE ? 2 : 1; }
+// units of one KV head
+__device__ __forceinline__ long long head_work(int vec, int blocks) {
+  const int rest = vec % 256;
+  return (long long)key_tiles(blocks) * (2 * (vec / 256) + (rest ? item_units(rest) : 0));
+}
+__device__ __forceinline__ long long cta_bound(long long work, int c, int ctas) { return work * c / ctas; }
+// Where the part of (CTA c, item) lies: twice the vectors of the items before it, and 256 for each
+// CTA before it; the part itself has at most 256, so that consecutive parts do not overlap.
+__device__ __forceinline__ long long prefix_offset(long long vec_at, int nkv, int h, int vec, int item, int cta) {
+  return 2 * (vec_at * nkv + (long long)h * vec + 256LL * item) + 256LL * cta;
+}
+
+// ---------------------------------------------------------------- prefixes: the tensor-core kernel
+constexpr int PRE_THREADS = 320;           // two softmax warpgroups, a load warp, an MMA warp
+constexpr int SLOT_BYTES = TILE * D * 2;   // one K or V tile: two halves of 64 dimensions, rows of 128 B
+constexpr int RING = 4;
+constexpr int TMEM_COLS = 512;             // S of both streams (their P in the same columns), O of both
+constexpr float RESCALE = 8.f;             // (log2) how far scores may pass the reference before it moves
+
+struct PrePlan {
+  int start[MAX_SEQS], at[MAX_SEQS];       // the entry's first row; its first row among its group's
+  int rows[MAX_SEQS];
+  short group[MAX_SEQS];
+  int group_rows[MAX_SEQS], group_first[MAX_SEQS];  // rows; a member (whose table is read)
+  long long work[MAX_SEQS + 1];
+};
+struct PreShared {
+  uint64_t full[RING], empty[RING], s_full[2], p_ready[2], q_ready[2], o_full[2];
+  uint32_t tmem;
+  volatile int abort_flag;
+  uint32_t valid[RING];                    // valid blocks of the tile in a slot
+};
+constexpr size_t PRE_SMEM = 1024 + 2 * SLOT_BYTES + RING * SLOT_BYTES + sizeof(PrePlan) + sizeof(PreShared);
+static_assert(PRE_SMEM <= 232448, "shared memory of one CTA");
+
+// D[tmem] (+)= A[tmem] B[smem]: the weights (bf16 pairs, a row per lane) times a V tile.
+__device__ __forceinline__ void tc_mma_bf16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// V as the B operand [keys][dimensions], dimensions contiguous: 64-dimension columns 16 KB apart, groups
+// of eight keys 1024 B apart, 128-byte swizzle.
+__device__ __forceinline__ uint64_t desc_v(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)((SLOT_BYTES / 2) >> 4) << 16) |
+         ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+constexpr uint32_t IDESC_QK = idesc_bf16_f32(TILE, TILE);
+constexpr uint32_t IDESC_PV = idesc_bf16_f32(TILE, D) | (1u << 16);  // B with its N dimension contiguous
+
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A CTA's part of one item: vectors [v0, v0 + nv) of (group, head), key tiles [t0, t1).
+struct Segment {
+  int group, h, item, v0, nv, t0, t1;
+};
+
+// Walks the segments of a CTA in order; every role walks them for itself.
+struct Walk {
+  const PrePlan* plan;
+  const int* group_blocks;  // device: prefix_blocks
+  long long lo, hi;
+  int groups, nkv, G;
+  int g, h, item;
+  long long at;  // units before the current item
+
+  __device__ Walk(const PrePlan* p, const ne_prefix_groups& pg, int nkv_, int G_, int cta, int ctas)
+      : plan(p), group_blocks(pg.prefix_blocks), groups(pg.num_groups), nkv(nkv_), G(G_) {
+    const long long work = p->work[groups];
+    lo = cta_bound(work, cta, ctas);
+    hi = cta_bound(work, cta + 1, ctas);
+    // the group, head and item that hold unit lo
+    int a = 0, b = groups;
+    while (a < b) {  // the last group whose work starts at or before lo
+      const int mid = (a + b + 1) >> 1;
+      if (p->work[mid] <= lo) a = mid;
+      else b = mid - 1;
+    }
+    g = min(a, max(groups - 1, 0));
+    h = 0;
+    item = 0;
+    at = p->work[g];
+    if (lo < hi) {
+      const int vec = p->group_rows[g] * G, blocks = group_blocks[g];
+      const long long hw = head_work(vec, blocks);
+      h = (int)((lo - at) / hw);
+      at += h * hw;
+      const long long per = 2LL * key_tiles(blocks);
+      item = (int)min((lo - at) / per, (long long)((vec - 1) / 256));
+      at += item * per;
+    }
+  }
+  __device__ bool next(Segment& s) {
+    while (at < hi && lo < hi) {
+      const int vec = plan->group_rows[g] * G;
+      if (vec == 0) {  // a group without rows has no work
+        ++g;
+        h = item = 0;
+        if (g >= groups) return false;
+        at = plan->work[g];
+        continue;
+      }
+      const int tiles = key_tiles(group_blocks[g]);
+      const int nv = min(256, vec - 256 * item), u = item_units(nv);
+      const long long from = lo > at ? lo - at : 0, to = hi - at;
+      const int t0 = (int)((from + u - 1) / u), t1 = (int)min((long long)tiles, (to + u - 1) / u);
+      s = Segment{g, h, item, 256 * item, nv, t0, t1};
+      at += (long long)u * tiles;
+      if (256 * (item + 1) < vec) {
+        ++item;
+      } else {
+        item = 0;
+        if (++h == nkv) {
+          h = 0;
+          ++g;
+          if (g >= groups) at = hi;  // the end of all work
+        }
+      }
+      if (t0 < t1) return true;
+    }
+    return false;
+  }
+};
+
+__global__ void __launch_bounds__(PRE_THREADS, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                  const __nv_bfloat16* __restrict__ q, ne_rows rows, ne_prefix_groups groups, int nh, int nkv,
+                  long long num_cache_slots, Parts parts, int* status) {
+  pdl_prologue();
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_s = smem;                              // [2 streams] query tiles
+  uint8_t* ring = smem + 2 * SLOT_BYTES;            // [RING] K and V tiles
+  PrePlan& plan = *reinterpret_cast<PrePlan*>(ring + RING * SLOT_BYTES);
+  PreShared& sh = *reinterpret_cast<PreShared*>(reinterpret_cast<uint8_t*>(&plan) + sizeof(PrePlan));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  const int G = nh / nkv, n = rows.num_seqs, ng = groups.num_groups;
+
+  // ---- barriers, tensor memory, and the plan
+  if (tid == 0) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sh.s_full[s], 1);
+      mbar_init(&sh.p_ready[s], 128);
+      mbar_init(&sh.q_ready[s], 128);
+      mbar_init(&sh.o_full[s], 1);
+    }
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&sh.tmem, TMEM_COLS);
+    tmem_relinquish();
+  }
+  for (int g = tid; g < ng; g += PRE_THREADS) {
+    plan.group_rows[g] = 0;
+    plan.group_first[g] = MAX_SEQS;
+  }
+  for (int b = tid; b < n; b += PRE_THREADS) {
+    const Entry e = entry_of(rows, groups, b, nullptr);  // (own_tokens_kernel reports what is refused)
+    plan.start[b] = e.start;
+    plan.rows[b] = e.rows;
+    plan.group[b] = (short)e.group;
+  }
+  __syncthreads();
+  for (int b = tid; b < n; b += PRE_THREADS) {
+    const int g = plan.group[b];
+    if (g < 0) continue;
+    int before = 0;
+    for (int x = 0; x < b; ++x) before += plan.group[x] == g ? plan.rows[x] : 0;
+    plan.at[b] = before;
+    atomicAdd(&plan.group_rows[g], plan.rows[b]);
+    atomicMin(&plan.group_first[g], b);
+    if (cta == 0) parts.entry_at[b] = before;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    long long work = 0, vecs = 0;
+    for (int g0 = 0; g0 < ng; g0 += 32) {
+      const int g = g0 + lane;
+      const int vec = g < ng ? plan.group_rows[g] * G : 0;
+      const long long w = vec ? nkv * head_work(vec, groups.prefix_blocks[g]) : 0;
+      long long wi = w, vi = vec;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long a = __shfl_up_sync(ALL, wi, o), c = __shfl_up_sync(ALL, vi, o);
+        if (lane >= o) {
+          wi += a;
+          vi += c;
+        }
+      }
+      if (g < ng) {
+        plan.work[g] = work + wi - w;
+        if (cta == 0) {
+          parts.group_work[g] = work + wi - w;
+          parts.group_vec[g] = vecs + vi - vec;
+        }
+      }
+      work += __shfl_sync(ALL, wi, 31);
+      vecs += __shfl_sync(ALL, vi, 31);
+    }
+    if (vecs > (long long)rows.max_rows * G) {  // entries that share rows: more parts than there is room for
+      if (lane == 0) report(status, NE_DEV_BAD_SLOT);
+      for (int g = lane; g < ng; g += 32) plan.work[g] = 0;
+      work = 0;
+    }
+    __syncwarp();
+    if (lane == 0) {
+      plan.work[ng] = work;
+      if (cta == 0) {
+        parts.group_work[ng] = work;
+        parts.group_vec[ng] = vecs;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  Walk walk(&plan, groups, nkv, G, cta, ctas);
+  Segment sg;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax of stream s, a row per thread
+    const int s = warp >> 2, row = tid & 127;
+    const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // 32 rows x (1 << 16)
+    const uint32_t t_s = tmem + lane_base + s * TILE, t_o = tmem + lane_base + 256 + s * D;
+    uint8_t* my_q = q_s + s * SLOT_BYTES;
+    uint32_t tile_phase = 0, o_phase = 0;
+    uint32_t slots_before = 0;  // tiles of K and V that earlier segments put through the ring
+    while (walk.next(sg)) {
+      const bool pair = sg.nv > TILE;
+      const int tiles = sg.t1 - sg.t0;
+      // the query tile: vector v of the group is head v % G of the group's row v / G
+      const int v = sg.v0 + (pair ? s * TILE : 0) + row;
+      const bool live = v < sg.v0 + sg.nv;
+      {
+        uint4 x[16];
+        const uint4* src = nullptr;
+        if (live) {
+          const int r = v / G;
+          int at = 0;
+          for (int b = 0; b < n; ++b)
+            if (plan.group[b] == sg.group && r >= plan.at[b] && r < plan.at[b] + plan.rows[b])
+              at = plan.start[b] + r - plan.at[b];
+          src = reinterpret_cast<const uint4*>(q + ((long long)at * nh + sg.h * G + v % G) * D);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          *reinterpret_cast<uint4*>(my_q + (i >> 3) * (SLOT_BYTES / 2) + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = x[i];
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.q_ready[s]);
+      float ref = NEG_INF, l = 0.f;
+      bool ok = true;
+      bool any = false;
+      for (int t = pair ? 0 : s; t < tiles; t += pair ? 1 : 2) {
+        ok = mbar_wait(&sh.s_full[s], tile_phase & 1u, &sh.abort_flag, status);
+        if (!__all_sync(ALL, ok)) {
+          ok = false;
+          break;
+        }
+        ++tile_phase;
+        tc_fence_after();
+        const uint32_t v_at = pair ? 2 * t + 1 : (uint32_t)min(2 * t + 2, 2 * tiles - 1);
+        float x[TILE];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_start(t_s + 32 * c, x + 32 * c);
+        // the mask comes with the V tile (K's slot may be refilled by now)
+        ok = mbar_wait(&sh.full[(slots_before + v_at) % RING], ((slots_before + v_at) / RING) & 1u, &sh.abort_flag,
+                       status);
+        const uint32_t valid = sh.valid[(slots_before + v_at) % RING];
+        tmem_ld_wait();
+        if (!__all_sync(ALL, ok)) {
+          ok = false;
+          break;
+        }
+        if (valid != 0xFFu) {
+#pragma unroll
+          for (int c = 0; c < TILE; ++c)
+            if (!(valid >> (c >> 4) & 1u)) x[c] = NEG_INF;
+        }
+        float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+        for (int c = 0; c < TILE; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * SCALE_LOG2;
+        // the reference moves only when the scores pass it by 2^8 (the sums stay far inside fp32)
+        if (__any_sync(ALL, top > ref + RESCALE)) {
+          const float next = fmaxf(ref, top);
+          const float f = ref == NEG_INF ? 0.f : ex2(ref - next);
+          ref = next;
+          l *= f;
+          if (any) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              tmem_ld32_start(t_o + 32 * c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= f;
+              tmem_st32(t_o + 32 * c, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+        }
+        any = true;
+        const float base = ref == NEG_INF ? 0.f : ref;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float p0 = ex2(fmaf(x[64 * c + 2 * i], SCALE_LOG2, -base));
+            const float p1 = ex2(fmaf(x[64 * c + 2 * i + 1], SCALE_LOG2, -base));
+            sum[(2 * i) & 3] += p0;
+            sum[(2 * i + 1) & 3] += p1;
+            p[i] = pack_bf16(p0, p1);
+          }
+          tmem_st32(t_s + 32 * c, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sh.p_ready[s]);
+      }
+      if (!ok) break;
+      // the part: the group's vectors from prefix_offset on; a lone tile's second stream 128 behind
+      const int vec = plan.group_rows[sg.group] * G;
+      long long vec_at = 0;
+      for (int g = 0; g < sg.group; ++g) vec_at += plan.group_rows[g] * G;
+      const long long at = prefix_offset(vec_at, nkv, sg.h, vec, sg.item, cta) +
+                           (pair ? s * TILE : s * sg.nv) + row;
+      if (any) {
+        ok = mbar_wait(&sh.o_full[s], o_phase & 1u, &sh.abort_flag, status);
+        if (!__all_sync(ALL, ok)) break;
+        ++o_phase;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tmem_ld32_start(t_o + 32 * c, o);
+          tmem_ld_wait();
+          if (live) {
+            float4* dst = reinterpret_cast<float4*>(parts.pre_o + at * D + 32 * c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+      if (live) {
+        parts.pre_m[at] = any ? ref : NEG_INF;
+        parts.pre_l[at] = l;
+      }
+      slots_before += 2 * tiles;
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ loads
+    uint32_t load = 0;  // ring slots filled
+    bool ok = true;
+    while (ok && walk.next(sg)) {
+      const bool pair = sg.nv > TILE;
+      const int tiles = sg.t1 - sg.t0, blocks = groups.prefix_blocks[sg.group];
+      const int32_t* table = table_of(rows, plan.group_first[sg.group]);
+      for (int i = 0; ok && i < 2 * tiles; ++i, ++load) {
+        // the order of use: K0 V0 K1 V1 .. for two query tiles, K0 K1 V0 K2 V1 .. for two key streams
+        bool is_v;
+        int t;
+        if (pair) {
+          is_v = i & 1;
+          t = i >> 1;
+        } else if (i == 2 * tiles - 1) {
+          is_v = true;
+          t = tiles - 1;
+        } else if (i == 0) {
+          is_v = false;
+          t = 0;
+        } else {
+          is_v = !(i & 1);
+          t = is_v ? (i >> 1) - 1 : (i + 1) >> 1;
+        }
+        const int slot = load % RING;
+        if (load >= RING) {
+          ok = mbar_wait(&sh.empty[slot], (load / RING - 1) & 1u, &sh.abort_flag, status);
+          ok = __all_sync(ALL, ok);
+          if (!ok) break;
+        }
+        // lanes 0-15: block lane / 2, half lane % 2 of the head dimension
+        const int kb = (sg.t0 + t) * 8 + (lane >> 1);
+        int id = -1;
+        if (lane < 16 && kb < blocks) {
+          id = table[kb];
+          if (id < 0 || (long long)(id + 1) * 16 > num_cache_slots - 1) {
+            report(status, NE_DEV_BAD_SLOT);
+            id = -1;
+          }
+        }
+        const uint32_t have = __ballot_sync(ALL, id >= 0);
+        uint32_t mask = 0;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) mask |= (have >> (2 * x) & 1u) << x;
+        if (lane == 0) {
+          sh.valid[slot] = mask;
+          if (mask) mbar_arrive_expect_tx(&sh.full[slot], __popc(have) * 2048);
+          else mbar_arrive(&sh.full[slot]);
+        }
+        __syncwarp();
+        if (id >= 0)
+          tma_load_3d(ring + slot * SLOT_BYTES + (lane & 1) * (SLOT_BYTES / 2) + (lane >> 1) * 2048,
+                      is_v ? &vmap : &kmap, &sh.full[slot], 64 * (lane & 1), sg.h, id * 16);
+      }
+    }
+    // (given up: the loads in flight land before the CTA leaves; the wait is bounded as all are)
+    if (!ok)
+      for (uint32_t i = load > RING ? load - RING : 0; i < load; ++i)
+        mbar_wait(&sh.full[i % RING], (i / RING) & 1u, nullptr, status);
+  } else {
+    // ------------------------------------------------------------ products (one thread issues)
+    uint32_t base = 0, q_phase = 0, p_phase[2] = {0, 0};
+    const uint32_t ring_u = smem_u32(ring), q_u = smem_u32(q_s);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && __all_sync(ALL, mbar_wait(bar, parity, &sh.abort_flag, status));
+      return ok;
+    };
+    auto full = [&](uint32_t at) { return wait(&sh.full[(base + at) % RING], ((base + at) / RING) & 1u); };
+    auto scores = [&](int s, uint32_t at) {  // S = Q K^T of stream s
+      if (lane == 0) {
+        const uint32_t k = ring_u + ((base + at) % RING) * SLOT_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t off = (kk >> 2) * (SLOT_BYTES / 2) + (kk & 3) * 32;
+          tc_mma_bf16(tmem + s * TILE, smem_desc_sw128(q_u + s * SLOT_BYTES + off), smem_desc_sw128(k + off), IDESC_QK,
+                      kk > 0);
+        }
+        tc_commit(&sh.s_full[s]);
+      }
+      __syncwarp();
+    };
+    bool begun[2] = {false, false};                       // the stream's O holds a product of this segment
+    auto values = [&](int s, uint32_t at) {               // O (+)= P V, the valid blocks only
+      if (lane == 0) {
+        const uint32_t v = ring_u + ((base + at) % RING) * SLOT_BYTES;
+        const uint32_t mask = sh.valid[(base + at) % RING];
+        bool acc = begun[s];
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          if (!(mask >> kk & 1u)) continue;
+          tc_mma_bf16_ta(tmem + 256 + s * D, tmem + s * TILE + 8 * kk, desc_v(v + kk * 2048), IDESC_PV, acc);
+          acc = true;
+        }
+        begun[s] = acc;
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (lane == 0) tc_commit(bar);
+      __syncwarp();
+    };
+    auto release = [&](uint32_t at) { commit(&sh.empty[(base + at) % RING]); };
+    while (ok && walk.next(sg)) {
+      const bool pair = sg.nv > TILE;
+      const int tiles = sg.t1 - sg.t0;
+      if (!wait(&sh.q_ready[0], q_phase & 1u) || !wait(&sh.q_ready[1], q_phase & 1u)) break;
+      ++q_phase;
+      begun[0] = begun[1] = false;
+      tc_fence_after();
+      if (pair) {
+        if (!full(0)) break;
+        scores(0, 0);
+        scores(1, 0);
+        release(0);
+        for (int t = 0; ok && t < tiles; ++t) {
+          if (!full(2 * t + 1)) break;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (!wait(&sh.p_ready[s], p_phase[s] & 1u)) break;
+            ++p_phase[s];
+            tc_fence_after();
+            values(s, 2 * t + 1);
+            if (s == 1) release(2 * t + 1);
+            if (t + 1 < tiles) {
+              if (!full(2 * t + 2)) break;
+              scores(s, 2 * t + 2);
+              if (s == 1) release(2 * t + 2);
+            } else {
+              commit(&sh.o_full[s]);
+            }
+          }
+        }
+      } else {
+        for (int s = 0; s < 2 && s < tiles; ++s) {
+          if (!full(s)) break;
+          scores(s, s);
+          release(s);
+        }
+        for (int t = 0; ok && t < tiles; ++t) {
+          const int s = t & 1;
+          const uint32_t v_at = (uint32_t)min(2 * t + 2, 2 * tiles - 1);
+          if (!full(v_at) || !wait(&sh.p_ready[s], p_phase[s] & 1u)) break;
+          ++p_phase[s];
+          tc_fence_after();
+          values(s, v_at);
+          release(v_at);
+          if (t + 2 < tiles) {
+            if (!full(2 * t + 3)) break;
+            scores(s, 2 * t + 3);
+            release(2 * t + 3);
+          } else {
+            commit(&sh.o_full[s]);
+          }
+        }
+      }
+      base += 2 * tiles;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// ---------------------------------------------------------------- the join
+constexpr int JOIN_WARPS = 8;
+
+// A warp per vector: four dimensions a lane.
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+    join_kernel(__nv_bfloat16* __restrict__ out, ne_rows rows, ne_prefix_groups groups, int nh, int nkv, Parts parts,
+                int pre_ctas) {
+  pdl_prologue();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
+  const Entry e = entry_of(rows, groups, b, nullptr);
+  const int x = blockIdx.y * JOIN_WARPS + warp;
+  if (x >= e.rows * nh) return;
+  const int j = x / nh, head = x % nh, G = nh / nkv, h = head / G;
+  const int row = e.start + j;
+  float m = NEG_INF, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float* po, float pm, float pl, long long at) {
+    if (pm == NEG_INF) return;  // (an empty part: its sums were never written)
+    const float mn = fmaxf(m, pm), f = m == NEG_INF ? 0.f : exp2f(m - mn), g = exp2f(pm - mn);
+    const float4 y = *reinterpret_cast<const float4*>(po + at * D + 4 * lane);
+    m = mn;
+    l = l * f + pl * g;
+    o = make_float4(o.x * f + y.x * g, o.y * f + y.y * g, o.z * f + y.z * g, o.w * f + y.w * g);
+  };
+  for (int s = 0; s < parts.splits; ++s) {
+    const long long at = ((long long)s * rows.max_rows + row) * nh + head;
+    add(parts.own_o, parts.own_m[at], parts.own_l[at], at);
+  }
+  const long long work = e.group >= 0 ? parts.group_work[groups.num_groups] : 0;
+  if (work > 0) {
+    const int g = e.group, blocks = groups.prefix_blocks[g], tiles = key_tiles(blocks);
+    const int vec = (int)(parts.group_vec[g + 1] - parts.group_vec[g]);
+    const int v = (parts.entry_at[b] + j) * G + head % G, item = v / 256;
+    const int nv = min(256, vec - 256 * item), u = item_units(nv);
+    const long long from = parts.group_work[g] + h * head_work(vec, blocks) + 2LL * tiles * item;
+    // the CTAs whose range meets the item's units
+    int c = (int)(from * pre_ctas / work);
+    while (c > 0 && cta_bound(work, c, pre_ctas) > from) --c;
+    while (cta_bound(work, c + 1, pre_ctas) <= from) ++c;
+    for (; c < pre_ctas && cta_bound(work, c, pre_ctas) < from + (long long)u * tiles; ++c) {
+      const long long lo = max(cta_bound(work, c, pre_ctas) - from, 0LL), hi = cta_bound(work, c + 1, pre_ctas) - from;
+      const int t0 = (int)((lo + u - 1) / u), t1 = (int)min((long long)tiles, (hi + u - 1) / u);
+      if (t0 >= t1) continue;
+      const long long base = prefix_offset(parts.group_vec[g], nkv, h, vec, item, c);
+      if (nv > TILE) {
+        const long long at = base + v - 256 * item;
+        add(parts.pre_o, parts.pre_m[at], parts.pre_l[at], at);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const long long at = base + s * nv + v - 256 * item;
+          add(parts.pre_o, parts.pre_m[at], parts.pre_l[at], at);
+        }
+      }
+    }
+  }
+  // (l is 0 only for a row that sees no key; NaN stays NaN)
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
+  *reinterpret_cast<uint2*>(out + ((long long)row * nh + head) * D + 4 * lane) = *reinterpret_cast<uint2*>(y);
+}
+
+int device_sms() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+// Splits of the entries' own tokens: one, unless the launch leaves most SMs idle and contexts are long
+// (32 blocks a split at least, as attention_plan_splits).
+int own_splits(int num_seqs, int nkv, int tiles, int max_context, int sms) {
+  const long long ctas = (long long)num_seqs * nkv * tiles;
+  long long splits = (2LL * sms + ctas - 1) / ctas;
+  splits = std::min<long long>(splits, max_context / 16 / 32);
+  return (int)std::max<long long>(1, std::min<long long>(splits, 16));
+}
+
+template <typename K>
+bool allow_smem(K kernel, size_t bytes, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (!done[dev])
+    done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+  return done[dev];
+}
+
+int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const void* k_cache, const void* v_cache,
+                            const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8,
+                            const ne_rows& rows, ne_prefix_groups groups, int nh, int nkv, long long slots,
+                            uint8_t* ws, size_t ws_bytes, int* status, cudaStream_t stream) {
+  const int sms = device_sms(), G = nh / nkv;
+  const int tiles = (int)(((long long)rows.max_q_len * G + 15) / 16);
+  const int splits = own_splits(rows.num_seqs, nkv, tiles, rows.max_context, sms);
+  const Layout l = layout_of(rows.max_rows, rows.num_seqs, groups.num_groups, nh, splits, sms);
+  if (ws_bytes < l.total) return NE_ERR_WORKSPACE;
+  if ((long long)tiles * splits > 65535 || nkv > 65535) return NE_ERR_UNSUPPORTED;
+  if (kv_int8 || groups.max_prefix_blocks == 0) groups.num_groups = 0;
+  auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
+  const Parts parts{f(l.own_o), f(l.own_m), f(l.own_l), f(l.pre_o), f(l.pre_m), f(l.pre_l),
+                    reinterpret_cast<int32_t*>(ws + l.entry_at), reinterpret_cast<long long*>(ws + l.group_work),
+                    reinterpret_cast<long long*>(ws + l.group_vec), splits};
+  static bool own_done[2][64] = {}, pre_done[64] = {};
+  auto own = kv_int8 ? own_tokens_kernel<true> : own_tokens_kernel<false>;
+  if (!allow_smem(own, OWN_SMEM, own_done[kv_int8 ? 1 : 0])) return NE_ERR_CUDA;
+  if (launch_kernel(own, dim3(rows.num_seqs, nkv, tiles * splits), dim3(32 * OWN_WARPS), OWN_SMEM, stream, q, k_cache,
+                    v_cache, k_scale, v_scale, rows, groups, nh, nkv, slots, parts, tiles, status) != cudaSuccess)
+    return NE_ERR_CUDA;
+  if (groups.num_groups > 0) {
+    CUtensorMap kmap, vmap;
+    if (!make_tmap_kv(&kmap, k_cache, nkv, slots) || !make_tmap_kv(&vmap, v_cache, nkv, slots)) return NE_ERR_CUDA;
+    if (!allow_smem(prefix_kernel, PRE_SMEM, pre_done)) return NE_ERR_CUDA;
+    if (launch_kernel(prefix_kernel, dim3(sms), dim3(PRE_THREADS), PRE_SMEM, stream, kmap, vmap, q, rows, groups, nh,
+                      nkv, slots, parts, status) != cudaSuccess)
+      return NE_ERR_CUDA;
+  }
+  const long long vectors = (long long)rows.max_q_len * nh;
+  return launch_kernel(join_kernel, dim3(rows.num_seqs, (unsigned)((vectors + JOIN_WARPS - 1) / JOIN_WARPS)),
+                       dim3(32 * JOIN_WARPS), 0, stream, out, rows, groups, nh, nkv, parts, sms) == cudaSuccess
+             ? NE_OK
+             : NE_ERR_CUDA;
+}
+
+bool heads_ok(int nh, int nkv) { return nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= MAX_GROUP; }
 
 }  // namespace
 
@@ -77,10 +1076,13 @@ __global__ void __launch_bounds__(128)
 
 extern "C" NE_API size_t ne_prefix_attention_workspace_bytes(int max_rows, int num_seqs, int num_groups, int num_heads,
                                                              int num_kv_heads, int max_q_len, int max_context) {
-  if (max_rows < 0 || num_seqs < 0 || num_seqs > 1024 || num_groups < 0 || num_kv_heads < 1 || num_heads < 1 ||
-      num_heads % num_kv_heads || num_heads / num_kv_heads > 32 || max_q_len < 0 || max_context < 0)
+  if (max_rows < 0 || num_seqs < 1 || num_seqs > ne::MAX_SEQS || num_groups < 0 || num_groups > ne::MAX_SEQS ||
+      !ne::heads_ok(num_heads, num_kv_heads) || max_q_len < 1 || max_context < 0)
     return 0;
-  return 256;
+  const int sms = ne::device_sms();
+  const int tiles = (int)(((long long)max_q_len * (num_heads / num_kv_heads) + 15) / 16);
+  return ne::layout_of(max_rows, num_seqs, num_groups, num_heads,
+                       ne::own_splits(num_seqs, num_kv_heads, tiles, max_context, sms), sms).total;
 }
 
 extern "C" NE_API int ne_prefix_attention(const void* q, void* out, const void* k_cache, const void* v_cache,
@@ -89,24 +1091,19 @@ extern "C" NE_API int ne_prefix_attention(const void* q, void* out, const void* 
                                           int block_size, long long num_cache_slots, void* workspace,
                                           size_t workspace_bytes, int32_t* status, void* stream) {
   if (!q || !out || !k_cache || !v_cache || !rows || !groups || (kv_int8 && (!k_scale || !v_scale)) ||
-      num_cache_slots < 2 || block_size != 16 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads ||
-      num_heads / num_kv_heads > 32 || rows->num_seqs <= 0 || rows->num_seqs > 1024 || rows->max_rows <= 0 ||
-      rows->max_q_len <= 0 || rows->max_context < 0 || rows->block_table_stride < 0 || !rows->positions ||
-      !rows->q_start || !rows->q_len || !rows->block_tables || groups->num_groups < 0 ||
-      groups->max_prefix_blocks < 0 || (groups->num_groups > 0 && (!groups->entry_group || !groups->prefix_blocks)))
+      num_cache_slots < 17 || block_size != 16 || !ne::heads_ok(num_heads, num_kv_heads) || rows->num_seqs <= 0 ||
+      rows->num_seqs > ne::MAX_SEQS || rows->max_rows <= 0 || rows->max_q_len <= 0 || rows->max_context < 0 ||
+      rows->block_table_stride < 0 || !rows->positions || !rows->q_start || !rows->q_len || !rows->block_tables ||
+      groups->num_groups < 0 || groups->num_groups > ne::MAX_SEQS || groups->max_prefix_blocks < 0 ||
+      (groups->num_groups > 0 && (!groups->entry_group || !groups->prefix_blocks)))
     return NE_ERR_INVALID;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return NE_ERR_INVALID;
-  const size_t need =
-      ne_prefix_attention_workspace_bytes(rows->max_rows, rows->num_seqs, groups->num_groups, num_heads, num_kv_heads,
-                                          rows->max_q_len, rows->max_context);
-  if (need == 0) return NE_ERR_INVALID;
-  if (workspace_bytes < need) return NE_ERR_WORKSPACE;
-  return ne::launch_kernel(ne::row_attention_kernel,
-                           dim3(rows->num_seqs, ((long long)rows->max_q_len * num_heads + 3) / 4), dim3(128), 0,
-                           static_cast<cudaStream_t>(stream), static_cast<const __nv_bfloat16*>(q),
-                           static_cast<__nv_bfloat16*>(out), k_cache, v_cache,
-                           static_cast<const __nv_bfloat16*>(k_scale), static_cast<const __nv_bfloat16*>(v_scale),
-                           kv_int8, *rows, num_heads, num_kv_heads, num_cache_slots, status) == cudaSuccess
-             ? NE_OK
-             : NE_ERR_CUDA;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) ||
+      ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 127u) || !workspace ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return NE_ERR_INVALID;
+  return ne::launch_prefix_attention(
+      static_cast<const __nv_bfloat16*>(q), static_cast<__nv_bfloat16*>(out), k_cache, v_cache,
+      static_cast<const __nv_bfloat16*>(k_scale), static_cast<const __nv_bfloat16*>(v_scale), kv_int8, *rows, *groups,
+      num_heads, num_kv_heads, num_cache_slots, static_cast<uint8_t*>(workspace), workspace_bytes, status,
+      static_cast<cudaStream_t>(stream));
 }
