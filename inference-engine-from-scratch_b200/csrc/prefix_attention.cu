@@ -30,8 +30,8 @@ struct Parts {
   float *pre_o, *pre_m, *pre_l;
   // the plan, written by prefix_kernel's first CTA for the join
   int32_t* entry_at;      // [num_seqs] the entry's first row among its group's
-  long long* group_work;  // [num_groups + 1] work before group g (its units: see Plan)
-  long long* group_vec;   // [num_groups + 1] vectors of one KV head before group g
+  int32_t* group_work;    // [num_groups + 1] units of work before group g
+  int32_t* group_vec;     // [num_groups + 1] vectors of one KV head before group g
   int splits;
 };
 
@@ -41,11 +41,8 @@ struct Layout {
   size_t own_o, own_m, own_l, pre_o, pre_m, pre_l, entry_at, group_work, group_vec, total;
 };
 
-// Vectors of the prefixes' parts: each item's twice (an item of one tile has two parts, one of two
-// tiles a part of each), and 256 more for every boundary between CTAs (see prefix_offset).
-inline long long prefix_part_vectors(long long max_rows, int nh, int ctas) {
-  return 2 * max_rows * nh + 256LL * (ctas + 1);
-}
+// Vectors of the prefixes' parts: every vector once, and 256 more for each CTA (see prefix_offset).
+inline long long prefix_part_vectors(long long max_rows, int nh, int ctas) { return max_rows * nh + 256LL * (ctas + 1); }
 
 inline Layout layout_of(long long max_rows, int num_seqs, int num_groups, int nh, int splits, int ctas) {
   Layout l;
@@ -64,8 +61,8 @@ inline Layout layout_of(long long max_rows, int num_seqs, int num_groups, int nh
   l.pre_m = take(pre * 4);
   l.pre_l = take(pre * 4);
   l.entry_at = take((size_t)num_seqs * 4);
-  l.group_work = take(((size_t)num_groups + 1) * 8);
-  l.group_vec = take(((size_t)num_groups + 1) * 8);
+  l.group_work = take(((size_t)num_groups + 1) * 4);
+  l.group_vec = take(((size_t)num_groups + 1) * 4);
   l.total = at;
   return l;
 }
@@ -95,6 +92,13 @@ __device__ __forceinline__ Entry entry_of(const ne_rows& rows, const ne_prefix_g
 
 __device__ __forceinline__ const int32_t* table_of(const ne_rows& rows, int b) {
   return rows.block_tables + (long long)(rows.table_index ? rows.table_index[b] : b) * rows.block_table_stride;
+}
+
+// The larger value; NaN if one is.
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 // ---------------------------------------------------------------- own tokens
@@ -136,15 +140,15 @@ __device__ __forceinline__ void own_block(TileState& ts, uint32_t k_s, uint32_t 
         masked |= ts.pos[r] >= 0;  // (a row without keys has no sums to keep clean)
       }
       s[j][e] = v;
-      mx[r] = fmaxf(mx[r], v);
+      mx[r] = max2(mx[r], v);
     }
   }
   float corr[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    mx[r] = fmaxf(mx[r], __shfl_xor_sync(ALL, mx[r], 1));
-    mx[r] = fmaxf(mx[r], __shfl_xor_sync(ALL, mx[r], 2));
-    const float m_new = fmaxf(ts.m[r], mx[r]);
+    mx[r] = max2(mx[r], __shfl_xor_sync(ALL, mx[r], 1));
+    mx[r] = max2(mx[r], __shfl_xor_sync(ALL, mx[r], 2));
+    const float m_new = max2(ts.m[r], mx[r]);
     corr[r] = (m_new == NEG_INF || ts.m[r] == NEG_INF) ? (m_new == NEG_INF ? 1.f : 0.f) : exp2f(ts.m[r] - m_new);
     ts.m[r] = m_new;
   }
@@ -373,45 +377,44 @@ __global__ void __launch_bounds__(32 * OWN_WARPS, 3)
 }
 
 // ---------------------------------------------------------------- prefixes: the division of the work
-// A group's vectors of one KV head are cut into items of up to 256. An item of more than 128 is two
-// query tiles that share every tile of 128 keys (2 units of work a key tile); a smaller one is one
-// query tile whose two halves of the SM take every second key tile (1 unit). The units of all (group,
-// head, item) in turn are divided evenly over the CTAs: CTA c does the key tiles that start in units
-// [c W / n, (c + 1) W / n).
-struct Group {
-  int vec, blocks;        // query vectors of one KV head, prefix blocks
-  long long work, vec_at;  // units before it; vectors (of one KV head) before it
-};
+// A group's vectors of one KV head are cut into items of up to 256: one or two query tiles, which share
+// every tile of 128 keys. A key tile costs an item 3 units of work with one query tile and 4 with two
+// (measured: about 1,900 and 2,500 cycles). The units of all (group, head, item) in turn are divided
+// evenly over the CTAs: CTA c does the key tiles that start in its ceil(W / CTAs) units from
+// c ceil(W / CTAs) on.
 __device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 7) / 8; }
-__device__ __forceinline__ int item_units(int vec) { return vec > TILE ? 2 : 1; }
+__device__ __forceinline__ int item_units(int vec) { return vec > TILE ? 4 : 3; }
 // units of one KV head
-__device__ __forceinline__ long long head_work(int vec, int blocks) {
+__device__ __forceinline__ int head_work(int vec, int blocks) {
   const int rest = vec % 256;
-  return (long long)key_tiles(blocks) * (2 * (vec / 256) + (rest ? item_units(rest) : 0));
+  return key_tiles(blocks) * (4 * (vec / 256) + (rest ? item_units(rest) : 0));
 }
-__device__ __forceinline__ long long cta_bound(long long work, int c, int ctas) { return work * c / ctas; }
-// Where the part of (CTA c, item) lies: twice the vectors of the items before it, and 256 for each
-// CTA before it; the part itself has at most 256, so that consecutive parts do not overlap.
+// Where the part of (CTA c, item) lies: behind the vectors of the items before it and 256 for each CTA
+// before it; a part has at most 256, so that consecutive ones do not overlap.
 __device__ __forceinline__ long long prefix_offset(long long vec_at, int nkv, int h, int vec, int item, int cta) {
-  return 2 * (vec_at * nkv + (long long)h * vec + 256LL * item) + 256LL * cta;
+  return vec_at * nkv + (long long)h * vec + 256LL * item + 256LL * cta;
 }
 
 // ---------------------------------------------------------------- prefixes: the tensor-core kernel
-constexpr int PRE_THREADS = 320;           // two softmax warpgroups, a load warp, an MMA warp
+constexpr int PRE_THREADS = 384;           // two softmax warpgroups; a load warp, two MMA warps, one idle
 constexpr int SLOT_BYTES = TILE * D * 2;   // one K or V tile: two halves of 64 dimensions, rows of 128 B
 constexpr int RING = 4;
-constexpr int TMEM_COLS = 512;             // S of both streams (their P in the same columns), O of both
+constexpr int HALF = TILE / 2;             // keys of a softmax step
+constexpr int TMEM_COLS = 512;             // two halves of S (P in the same columns) and O for each query tile
+constexpr int POLY_PAIRS = 3;              // of 8 pairs of weights, those whose 2^x runs on the FMA pipe
 constexpr float RESCALE = 8.f;             // (log2) how far scores may pass the reference before it moves
 
-struct PrePlan {
+struct alignas(16) PrePlan {
+  uint32_t key[MAX_SEQS];                  // rows << 12 | group + 1 (0: none)
   int start[MAX_SEQS], at[MAX_SEQS];       // the entry's first row; its first row among its group's
-  int rows[MAX_SEQS];
-  short group[MAX_SEQS];
-  int group_rows[MAX_SEQS], group_first[MAX_SEQS];  // rows; a member (whose table is read)
-  long long work[MAX_SEQS + 1];
+  short member[MAX_SEQS];                  // the groups' entries in order, group by group
+  int group_first[MAX_SEQS];               // the first of the group's members
+  int work[MAX_SEQS + 1], vec[MAX_SEQS + 1];        // units, and vectors of one KV head, before the group
+  int blocks[MAX_SEQS];                    // prefix_blocks
+  int members;
 };
-struct PreShared {
-  uint64_t full[RING], empty[RING], s_full[2], p_ready[2], q_ready[2], o_full[2];
+struct alignas(16) PreShared {
+  uint64_t full[RING], empty[RING], s_full[2][2], p_ready[2][2], o_done[2][2], q_ready[2];
   uint32_t tmem;
   volatile int abort_flag;
   uint32_t valid[RING];                    // valid blocks of the tile in a slot
@@ -435,7 +438,7 @@ __device__ __forceinline__ uint64_t desc_v(uint32_t smem_addr) {
   return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)((SLOT_BYTES / 2) >> 4) << 16) |
          ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
 }
-constexpr uint32_t IDESC_QK = idesc_bf16_f32(TILE, TILE);
+constexpr uint32_t IDESC_QK = idesc_bf16_f32(TILE, HALF);
 constexpr uint32_t IDESC_PV = idesc_bf16_f32(TILE, D) | (1u << 16);  // B with its N dimension contiguous
 
 __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float* v) {
@@ -470,6 +473,60 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^t for two finite t up to 126 (below -126: 2^-126), on the FMA pipe beside the special-function one:
+// t = n + f, n = rint(t) read off the low bits of t + 1.5 x 2^23, and 2^f on [-1/2, 1/2] by the cubic
+// whose largest relative error is least (7.5e-5; the weight is rounded to bf16, 2^-9, next).
+__device__ __forceinline__ void ex2_poly(uint64_t t2, float& a, float& b) {
+  unpack2(t2, a, b);
+  t2 = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  constexpr float MAGIC = 12582912.f;
+  constexpr float C0 = 0.99992806f, C1 = 0.69326097f, C2 = 0.24261113f, C3 = 0.05517165f;
+  const uint64_t n2 = add2(t2, pack2(MAGIC, MAGIC));
+  const uint64_t f2 = fma2(add2(n2, pack2(-MAGIC, -MAGIC)), pack2(-1.f, -1.f), t2);
+  uint64_t y2 = fma2(f2, pack2(C3, C3), pack2(C2, C2));
+  y2 = fma2(y2, f2, pack2(C1, C1));
+  y2 = fma2(y2, f2, pack2(C0, C0));
+  float na, nb;
+  unpack2(n2, na, nb);
+  unpack2(y2, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
+}
+
 // A CTA's part of one item: vectors [v0, v0 + nv) of (group, head), key tiles [t0, t1).
 struct Segment {
   int group, h, item, v0, nv, t0, t1;
@@ -478,18 +535,15 @@ struct Segment {
 // Walks the segments of a CTA in order; every role walks them for itself.
 struct Walk {
   const PrePlan* plan;
-  const int* group_blocks;  // device: prefix_blocks
-  long long lo, hi;
   int groups, nkv, G;
-  int g, h, item;
-  long long at;  // units before the current item
+  int lo, hi;               // the CTA's units
+  int g, h, item, at;       // the current item, and the units before it
 
-  __device__ Walk(const PrePlan* p, const ne_prefix_groups& pg, int nkv_, int G_, int cta, int ctas)
-      : plan(p), group_blocks(pg.prefix_blocks), groups(pg.num_groups), nkv(nkv_), G(G_) {
-    const long long work = p->work[groups];
-    lo = cta_bound(work, cta, ctas);
-    hi = cta_bound(work, cta + 1, ctas);
-    // the group, head and item that hold unit lo
+  __device__ Walk(const PrePlan* p, const ne_prefix_groups& pg, int nkv_, int G_, int per)
+      : plan(p), groups(pg.num_groups), nkv(nkv_), G(G_) {
+    const int work = p->work[groups];
+    lo = min(work, (int)blockIdx.x * per);
+    hi = min(work, lo + per);
     int a = 0, b = groups;
     while (a < b) {  // the last group whose work starts at or before lo
       const int mid = (a + b + 1) >> 1;
@@ -501,18 +555,18 @@ struct Walk {
     item = 0;
     at = p->work[g];
     if (lo < hi) {
-      const int vec = p->group_rows[g] * G, blocks = group_blocks[g];
-      const long long hw = head_work(vec, blocks);
-      h = (int)((lo - at) / hw);
+      const int vec = p->vec[g + 1] - p->vec[g], blocks = plan->blocks[g];
+      const int hw = head_work(vec, blocks);
+      h = (lo - at) / hw;
       at += h * hw;
-      const long long per = 2LL * key_tiles(blocks);
-      item = (int)min((lo - at) / per, (long long)((vec - 1) / 256));
-      at += item * per;
+      const int units = 4 * key_tiles(blocks);
+      item = min((lo - at) / units, (vec - 1) / 256);
+      at += item * units;
     }
   }
   __device__ bool next(Segment& s) {
     while (at < hi && lo < hi) {
-      const int vec = plan->group_rows[g] * G;
+      const int vec = plan->vec[g + 1] - plan->vec[g];
       if (vec == 0) {  // a group without rows has no work
         ++g;
         h = item = 0;
@@ -520,12 +574,12 @@ struct Walk {
         at = plan->work[g];
         continue;
       }
-      const int tiles = key_tiles(group_blocks[g]);
+      const int tiles = key_tiles(plan->blocks[g]);
       const int nv = min(256, vec - 256 * item), u = item_units(nv);
-      const long long from = lo > at ? lo - at : 0, to = hi - at;
-      const int t0 = (int)((from + u - 1) / u), t1 = (int)min((long long)tiles, (to + u - 1) / u);
+      const int from = max(lo - at, 0), to = hi - at;
+      const int t0 = (from + u - 1) / u, t1 = min(tiles, (to + u - 1) / u);
       s = Segment{g, h, item, 256 * item, nv, t0, t1};
-      at += (long long)u * tiles;
+      at += u * tiles;
       if (256 * (item + 1) < vec) {
         ++item;
       } else {
@@ -554,20 +608,21 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
   PrePlan& plan = *reinterpret_cast<PrePlan*>(ring + RING * SLOT_BYTES);
   PreShared& sh = *reinterpret_cast<PreShared*>(reinterpret_cast<uint8_t*>(&plan) + sizeof(PrePlan));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int cta = blockIdx.x, ctas = gridDim.x;
   const int G = nh / nkv, n = rows.num_seqs, ng = groups.num_groups;
 
   // ---- barriers, tensor memory, and the plan
   if (tid == 0) {
     for (int i = 0; i < RING; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.empty[i], 2);  // a release by each query tile's products
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&sh.s_full[s], 1);
-      mbar_init(&sh.p_ready[s], 128);
+      for (int half = 0; half < 2; ++half) {
+        mbar_init(&sh.s_full[s][half], 1);
+        mbar_init(&sh.p_ready[s][half], 128);
+        mbar_init(&sh.o_done[s][half], 1);
+      }
       mbar_init(&sh.q_ready[s], 128);
-      mbar_init(&sh.o_full[s], 1);
     }
     sh.abort_flag = 0;
     fence_mbar_init();
@@ -577,146 +632,187 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
     tmem_relinquish();
   }
   for (int g = tid; g < ng; g += PRE_THREADS) {
-    plan.group_rows[g] = 0;
-    plan.group_first[g] = MAX_SEQS;
+    plan.vec[g] = 0;          // (rows, until they are summed)
+    plan.group_first[g] = 0;  // (members, until their offsets are known)
+    plan.blocks[g] = groups.prefix_blocks[g];
   }
-  for (int b = tid; b < n; b += PRE_THREADS) {
-    const Entry e = entry_of(rows, groups, b, nullptr);  // (own_tokens_kernel reports what is refused)
+  for (int b = tid; b < (n + 3 & ~3); b += PRE_THREADS) {
+    const Entry e = b < n ? entry_of(rows, groups, b, nullptr) : Entry{0, 0, -1};  // (own_tokens_kernel reports)
     plan.start[b] = e.start;
-    plan.rows[b] = e.rows;
-    plan.group[b] = (short)e.group;
+    plan.key[b] = e.group >= 0 ? (uint32_t)e.rows << 12 | (uint32_t)(e.group + 1) : 0u;
   }
   __syncthreads();
-  for (int b = tid; b < n; b += PRE_THREADS) {
-    const int g = plan.group[b];
-    if (g < 0) continue;
+  int rank[(MAX_SEQS + PRE_THREADS - 1) / PRE_THREADS];  // members of the group before the entry
+#pragma unroll
+  for (int i = 0; i < (MAX_SEQS + PRE_THREADS - 1) / PRE_THREADS; ++i) {
+    const int b = tid + i * PRE_THREADS;
+    rank[i] = 0;
+    const uint32_t key = b < n ? plan.key[b] : 0u;
+    if (key == 0u) continue;
     int before = 0;
-    for (int x = 0; x < b; ++x) before += plan.group[x] == g ? plan.rows[x] : 0;
+    auto count = [&](uint32_t other, int x) {
+      if (x < b && ((other ^ key) & 0xFFFu) == 0u) {
+        before += other >> 12;
+        ++rank[i];
+      }
+    };
+    for (int x = 0; x < b; x += 4) {
+      const uint4 k4 = *reinterpret_cast<const uint4*>(&plan.key[x]);
+      count(k4.x, x);
+      count(k4.y, x + 1);
+      count(k4.z, x + 2);
+      count(k4.w, x + 3);
+    }
     plan.at[b] = before;
-    atomicAdd(&plan.group_rows[g], plan.rows[b]);
-    atomicMin(&plan.group_first[g], b);
-    if (cta == 0) parts.entry_at[b] = before;
+    const int g = (int)(key & 0xFFFu) - 1;
+    atomicAdd(&plan.vec[g], (int)(key >> 12));
+    atomicAdd(&plan.group_first[g], 1);
+    if (blockIdx.x == 0) parts.entry_at[b] = before;
   }
   __syncthreads();
   if (warp == 0) {
-    long long work = 0, vecs = 0;
+    int work = 0, vecs = 0, members = 0;
     for (int g0 = 0; g0 < ng; g0 += 32) {
       const int g = g0 + lane;
-      const int vec = g < ng ? plan.group_rows[g] * G : 0;
-      const long long w = vec ? nkv * head_work(vec, groups.prefix_blocks[g]) : 0;
-      long long wi = w, vi = vec;
+      const int vec = g < ng ? plan.vec[g] * G : 0, count = g < ng ? plan.group_first[g] : 0;
+      const int w = vec ? nkv * head_work(vec, plan.blocks[g]) : 0;
+      int wi = w, vi = vec, mi = count;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long a = __shfl_up_sync(ALL, wi, o), c = __shfl_up_sync(ALL, vi, o);
+        const int a = __shfl_up_sync(ALL, wi, o), c = __shfl_up_sync(ALL, vi, o), d = __shfl_up_sync(ALL, mi, o);
         if (lane >= o) {
           wi += a;
           vi += c;
+          mi += d;
         }
       }
       if (g < ng) {
         plan.work[g] = work + wi - w;
-        if (cta == 0) {
-          parts.group_work[g] = work + wi - w;
-          parts.group_vec[g] = vecs + vi - vec;
-        }
+        plan.vec[g] = vecs + vi - vec;
+        plan.group_first[g] = members + mi - count;
       }
       work += __shfl_sync(ALL, wi, 31);
       vecs += __shfl_sync(ALL, vi, 31);
+      members += __shfl_sync(ALL, mi, 31);
     }
-    if (vecs > (long long)rows.max_rows * G) {  // entries that share rows: more parts than there is room for
+    __syncwarp();
+    if (vecs > rows.max_rows * G) {  // entries that share rows: more parts than there is room for
       if (lane == 0) report(status, NE_DEV_BAD_SLOT);
       for (int g = lane; g < ng; g += 32) plan.work[g] = 0;
       work = 0;
     }
-    __syncwarp();
     if (lane == 0) {
       plan.work[ng] = work;
-      if (cta == 0) {
-        parts.group_work[ng] = work;
-        parts.group_vec[ng] = vecs;
-      }
+      plan.vec[ng] = vecs;
+      plan.members = members;
     }
+    __syncwarp();
+    if (blockIdx.x == 0)
+      for (int g = lane; g <= ng; g += 32) {
+        parts.group_work[g] = plan.work[g];
+        parts.group_vec[g] = plan.vec[g];
+      }
   }
   tc_fence_before();
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < (MAX_SEQS + PRE_THREADS - 1) / PRE_THREADS; ++i) {
+    const int b = tid + i * PRE_THREADS;
+    if (b < n && plan.key[b]) plan.member[plan.group_first[(plan.key[b] & 0xFFFu) - 1] + rank[i]] = (short)b;
+  }
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  Walk walk(&plan, groups, nkv, G, cta, ctas);
+  const int per = (plan.work[ng] + gridDim.x - 1) / gridDim.x;
+  Walk walk(&plan, groups, nkv, G, per);
   Segment sg;
 
   if (warp < 8) {
-    // ------------------------------------------------------------ softmax of stream s, a row per thread
+    // ------------------------------------------------------------ softmax of query tile s, a row per thread
     const int s = warp >> 2, row = tid & 127;
     const uint32_t lane_base = (uint32_t)(warp & 3) << 21;  // 32 rows x (1 << 16)
     const uint32_t t_s = tmem + lane_base + s * TILE, t_o = tmem + lane_base + 256 + s * D;
     uint8_t* my_q = q_s + s * SLOT_BYTES;
-    uint32_t tile_phase = 0, o_phase = 0;
-    uint32_t slots_before = 0;  // tiles of K and V that earlier segments put through the ring
+    uint32_t tiles_before = 0, slots_before = 0;  // key tiles of earlier segments: this warpgroup's, all
     while (walk.next(sg)) {
-      const bool pair = sg.nv > TILE;
       const int tiles = sg.t1 - sg.t0;
+      if (s == 1 && sg.nv <= TILE) {  // one query tile: the second warpgroup sits this segment out
+        slots_before += tiles;
+        continue;
+      }
       // the query tile: vector v of the group is head v % G of the group's row v / G
-      const int v = sg.v0 + (pair ? s * TILE : 0) + row;
+      const int v = sg.v0 + s * TILE + row;
       const bool live = v < sg.v0 + sg.nv;
       {
-        uint4 x[16];
-        const uint4* src = nullptr;
+        int at = -1;  // the row of q, in units of vectors
         if (live) {
           const int r = v / G;
-          int at = 0;
-          for (int b = 0; b < n; ++b)
-            if (plan.group[b] == sg.group && r >= plan.at[b] && r < plan.at[b] + plan.rows[b])
-              at = plan.start[b] + r - plan.at[b];
-          src = reinterpret_cast<const uint4*>(q + ((long long)at * nh + sg.h * G + v % G) * D);
+          int a = plan.group_first[sg.group];
+          int z = (sg.group + 1 < ng ? plan.group_first[sg.group + 1] : plan.members) - 1;
+          while (a < z) {  // the last member whose rows start at or before r
+            const int mid = (a + z + 1) >> 1;
+            if (plan.at[plan.member[mid]] <= r) a = mid;
+            else z = mid - 1;
+          }
+          const int b = plan.member[a];
+          at = (plan.start[b] + r - plan.at[b]) * nh + sg.h * G + v % G;
+        }
+        // half a warp a vector: 16 bytes a lane
+        const int ch = lane & 15;
+        uint4 x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int from = __shfl_sync(ALL, at, 2 * i + (lane >> 4));
+          x[i] = from >= 0 ? *reinterpret_cast<const uint4*>(q + (long long)from * D + 8 * ch) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          *reinterpret_cast<uint4*>(my_q + (i >> 3) * (SLOT_BYTES / 2) + row * 128 + (((i & 7) ^ (row & 7)) << 4)) = x[i];
+        for (int i = 0; i < 16; ++i) {
+          const int r = (warp & 3) * 32 + 2 * i + (lane >> 4);
+          *reinterpret_cast<uint4*>(my_q + (ch >> 3) * (SLOT_BYTES / 2) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[i];
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_ready[s]);
       float ref = NEG_INF, l = 0.f;
       bool ok = true;
-      bool any = false;
-      for (int t = pair ? 0 : s; t < tiles; t += pair ? 1 : 2) {
-        ok = mbar_wait(&sh.s_full[s], tile_phase & 1u, &sh.abort_flag, status);
-        if (!__all_sync(ALL, ok)) {
-          ok = false;
-          break;
-        }
-        ++tile_phase;
+      for (int j = 0; j < 2 * tiles; ++j) {  // 64 keys a step, S in two buffers: the next half's scores
+        const int t = j >> 1, half = j & 1;  // are computed while this one's weights are
+        ok = mbar_wait(&sh.s_full[s][half], (tiles_before + t) & 1u, &sh.abort_flag, status);
         tc_fence_after();
-        const uint32_t v_at = pair ? 2 * t + 1 : (uint32_t)min(2 * t + 2, 2 * tiles - 1);
-        float x[TILE];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_start(t_s + 32 * c, x + 32 * c);
+        float x[HALF];
+        tmem_ld32_start(t_s + HALF * half, x);
+        tmem_ld32_start(t_s + HALF * half + 32, x + 32);
         // the mask comes with the V tile (K's slot may be refilled by now)
-        ok = mbar_wait(&sh.full[(slots_before + v_at) % RING], ((slots_before + v_at) / RING) & 1u, &sh.abort_flag,
-                       status);
-        const uint32_t valid = sh.valid[(slots_before + v_at) % RING];
+        const uint32_t v_at = 2 * (slots_before + t) + 1;
+        ok = ok && mbar_wait(&sh.full[v_at % RING], (v_at / RING) & 1u, &sh.abort_flag, status);
+        const uint32_t valid = sh.valid[v_at % RING] >> (4 * half) & 0xFu;
         tmem_ld_wait();
-        if (!__all_sync(ALL, ok)) {
-          ok = false;
-          break;
-        }
-        if (valid != 0xFFu) {
+        if (valid != 0xFu) {
 #pragma unroll
-          for (int c = 0; c < TILE; ++c)
+          for (int c = 0; c < HALF; ++c)
             if (!(valid >> (c >> 4) & 1u)) x[c] = NEG_INF;
         }
-        float mx[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+        float mx[8];
 #pragma unroll
-        for (int c = 0; c < TILE; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * SCALE_LOG2;
+        for (int i = 0; i < 8; ++i) mx[i] = max3(x[i], x[8 + i], x[16 + i]);
+#pragma unroll
+        for (int c = 24; c < 56; c += 16)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx[i] = max3(mx[i], x[c + i], x[c + 8 + i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx[i] = max2(mx[i], x[56 + i]);
+        const float top =
+            max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max2(mx[6], mx[7])) * SCALE_LOG2;
+        const bool odd = __any_sync(ALL, !(fabsf(top) < INFINITY));  // NaN or infinite scores among them
         // the reference moves only when the scores pass it by 2^8 (the sums stay far inside fp32)
-        if (__any_sync(ALL, top > ref + RESCALE)) {
-          const float next = fmaxf(ref, top);
+        if (__any_sync(ALL, !(top <= ref + RESCALE))) {
+          const float next = max2(ref, top);
           const float f = ref == NEG_INF ? 0.f : ex2(ref - next);
           ref = next;
           l *= f;
-          if (any) {
+          if (t + half > 0) {  // O must hold the product of the step before, which may still run
+            ok = ok && mbar_wait(&sh.o_done[s][half ^ 1], (tiles_before + t - 1 + half) & 1u, &sh.abort_flag, status);
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               float o[32];
@@ -728,218 +824,206 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
             }
           }
         }
-        any = true;
         const float base = ref == NEG_INF ? 0.f : ref;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = pack2(SCALE_LOG2, SCALE_LOG2), base2 = pack2(-base, -base);
+        uint64_t sum[2] = {0ull, 0ull};  // (pairs of fp32 zeros)
+        uint32_t p[HALF / 2];
+        auto weigh = [&](bool all) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t p[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float p0 = ex2(fmaf(x[64 * c + 2 * i], SCALE_LOG2, -base));
-            const float p1 = ex2(fmaf(x[64 * c + 2 * i + 1], SCALE_LOG2, -base));
-            sum[(2 * i) & 3] += p0;
-            sum[(2 * i + 1) & 3] += p1;
-            p[i] = pack_bf16(p0, p1);
+          for (int i = 0; i < HALF / 2; ++i) {
+            float a, b;
+            const uint64_t t2 = fma2(pack2(x[2 * i], x[2 * i + 1]), scale2, base2);
+            if (all || i % 8 >= POLY_PAIRS) {
+              unpack2(t2, a, b);
+              a = ex2(a);
+              b = ex2(b);
+            } else {
+              ex2_poly(t2, a, b);
+            }
+            sum[i & 1] = add2(sum[i & 1], pack2(a, b));
+            p[i] = pack_bf16(a, b);
           }
-          tmem_st32(t_s + 32 * c, p);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        };
+        if (odd) weigh(true);
+        else weigh(false);
+        tmem_st32(t_s + HALF * half, p);
+        float s0, s1;
+        unpack2(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&sh.p_ready[s]);
+        mbar_arrive(&sh.p_ready[s][half]);
+        if (!__all_sync(ALL, ok)) {
+          ok = false;
+          break;
+        }
       }
       if (!ok) break;
-      // the part: the group's vectors from prefix_offset on; a lone tile's second stream 128 behind
-      const int vec = plan.group_rows[sg.group] * G;
-      long long vec_at = 0;
-      for (int g = 0; g < sg.group; ++g) vec_at += plan.group_rows[g] * G;
-      const long long at = prefix_offset(vec_at, nkv, sg.h, vec, sg.item, cta) +
-                           (pair ? s * TILE : s * sg.nv) + row;
-      if (any) {
-        ok = mbar_wait(&sh.o_full[s], o_phase & 1u, &sh.abort_flag, status);
-        if (!__all_sync(ALL, ok)) break;
-        ++o_phase;
-        tc_fence_after();
+      tiles_before += tiles;
+      slots_before += tiles;
+      // the part: unnormalised sums, and the reference and sum of their weights
+      const long long part = prefix_offset(plan.vec[sg.group], nkv, sg.h, plan.vec[sg.group + 1] - plan.vec[sg.group],
+                                           sg.item, blockIdx.x) + s * TILE;
+      const long long at = part + row;
+      ok = mbar_wait(&sh.o_done[s][1], (tiles_before - 1) & 1u, &sh.abort_flag, status);
+      if (!__all_sync(ALL, ok)) break;
+      tc_fence_after();
+      // O through shared memory (the warp's own rows of the query tile, whose products are done), 64
+      // dimensions at a time, so that half a warp writes 256 consecutive bytes
+      const int r0 = (warp & 3) * 32, rows_live = min(32, sg.nv - s * TILE - r0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          tmem_ld32_start(t_o + 32 * c, o);
-          tmem_ld_wait();
-          if (live) {
-            float4* dst = reinterpret_cast<float4*>(parts.pre_o + at * D + 32 * c);
+      for (int c = 0; c < 2; ++c) {
+        float o[64];
+        tmem_ld32_start(t_o + 64 * c, o);
+        tmem_ld32_start(t_o + 64 * c + 32, o + 32);
+        tmem_ld_wait();
+        __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
+        for (int i = 0; i < 16; ++i)
+          *reinterpret_cast<float4*>(my_q + (i >> 3) * (SLOT_BYTES / 2) + row * 128 + (((i & 7) ^ (row & 7)) << 4)) =
+              make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+        const int ch = lane & 15;
+        for (int r = lane >> 4; r < rows_live; r += 2) {
+          const float4 y = *reinterpret_cast<const float4*>(my_q + (ch >> 3) * (SLOT_BYTES / 2) + (r0 + r) * 128 +
+                                                            (((ch & 7) ^ (r & 7)) << 4));
+          *reinterpret_cast<float4*>(parts.pre_o + (part + r0 + r) * D + 64 * c + 4 * ch) = y;
         }
-        tc_fence_before();
       }
+      tc_fence_before();
       if (live) {
-        parts.pre_m[at] = any ? ref : NEG_INF;
+        parts.pre_m[at] = ref;
         parts.pre_l[at] = l;
       }
-      slots_before += 2 * tiles;
     }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------ loads
+  } else if (warp == 8 && elect_one()) {
+    // ------------------------------------------------------------ loads, issued by one thread
     uint32_t load = 0;  // ring slots filled
     bool ok = true;
     while (ok && walk.next(sg)) {
-      const bool pair = sg.nv > TILE;
-      const int tiles = sg.t1 - sg.t0, blocks = groups.prefix_blocks[sg.group];
-      const int32_t* table = table_of(rows, plan.group_first[sg.group]);
-      for (int i = 0; ok && i < 2 * tiles; ++i, ++load) {
-        // the order of use: K0 V0 K1 V1 .. for two query tiles, K0 K1 V0 K2 V1 .. for two key streams
-        bool is_v;
-        int t;
-        if (pair) {
-          is_v = i & 1;
-          t = i >> 1;
-        } else if (i == 2 * tiles - 1) {
-          is_v = true;
-          t = tiles - 1;
-        } else if (i == 0) {
-          is_v = false;
-          t = 0;
-        } else {
-          is_v = !(i & 1);
-          t = is_v ? (i >> 1) - 1 : (i + 1) >> 1;
+      const int blocks = plan.blocks[sg.group];
+      const int32_t* table = table_of(rows, plan.member[plan.group_first[sg.group]]);
+      int next[8];  // the next tile's block ids, loaded a tile ahead
+      auto look = [&](int t) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int kb = t * 8 + x;
+          next[x] = t < sg.t1 && kb < blocks ? table[kb] : -1;
         }
-        const int slot = load % RING;
-        if (load >= RING) {
-          ok = mbar_wait(&sh.empty[slot], (load / RING - 1) & 1u, &sh.abort_flag, status);
-          ok = __all_sync(ALL, ok);
-          if (!ok) break;
-        }
-        // lanes 0-15: block lane / 2, half lane % 2 of the head dimension
-        const int kb = (sg.t0 + t) * 8 + (lane >> 1);
-        int id = -1;
-        if (lane < 16 && kb < blocks) {
-          id = table[kb];
-          if (id < 0 || (long long)(id + 1) * 16 > num_cache_slots - 1) {
-            report(status, NE_DEV_BAD_SLOT);
-            id = -1;
-          }
-        }
-        const uint32_t have = __ballot_sync(ALL, id >= 0);
+      };
+      look(sg.t0);
+      for (int t = sg.t0; ok && t < sg.t1; ++t) {  // K0 V0 K1 V1 ..
+        int id[8];
         uint32_t mask = 0;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) mask |= (have >> (2 * x) & 1u) << x;
-        if (lane == 0) {
-          sh.valid[slot] = mask;
-          if (mask) mbar_arrive_expect_tx(&sh.full[slot], __popc(have) * 2048);
-          else mbar_arrive(&sh.full[slot]);
+        for (int x = 0; x < 8; ++x) {
+          id[x] = next[x];
+          if (id[x] >= 0 && (long long)(id[x] + 1) * 16 <= num_cache_slots - 1) mask |= 1u << x;
+          else if (t * 8 + x < blocks) report(status, NE_DEV_BAD_SLOT);
         }
-        __syncwarp();
-        if (id >= 0)
-          tma_load_3d(ring + slot * SLOT_BYTES + (lane & 1) * (SLOT_BYTES / 2) + (lane >> 1) * 2048,
-                      is_v ? &vmap : &kmap, &sh.full[slot], 64 * (lane & 1), sg.h, id * 16);
+        look(t + 1);
+        for (int is_v = 0; is_v < 2; ++is_v, ++load) {
+          const int slot = load % RING;
+          if (load >= RING) {
+            ok = mbar_wait(&sh.empty[slot], (load / RING - 1) & 1u, &sh.abort_flag, status);
+            if (!ok) break;
+          }
+          sh.valid[slot] = mask;
+          mbar_arrive_expect_tx(&sh.full[slot], __popc(mask) * 4096);
+          uint8_t* dst = ring + slot * SLOT_BYTES;
+          const CUtensorMap* map = is_v ? &vmap : &kmap;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            if (!(mask >> x & 1u)) continue;
+            tma_load_3d(dst + x * 2048, map, &sh.full[slot], 0, sg.h, id[x] * 16);
+            tma_load_3d(dst + SLOT_BYTES / 2 + x * 2048, map, &sh.full[slot], 64, sg.h, id[x] * 16);
+          }
+        }
       }
     }
     // (given up: the loads in flight land before the CTA leaves; the wait is bounded as all are)
     if (!ok)
       for (uint32_t i = load > RING ? load - RING : 0; i < load; ++i)
         mbar_wait(&sh.full[i % RING], (i / RING) & 1u, nullptr, status);
-  } else {
-    // ------------------------------------------------------------ products (one thread issues)
-    uint32_t base = 0, q_phase = 0, p_phase[2] = {0, 0};
-    const uint32_t ring_u = smem_u32(ring), q_u = smem_u32(q_s);
+  } else if ((warp == 9 || warp == 10) && elect_one()) {
+    // ------------------------------------------------------------ products of query tile s, issued by one thread
+    const int s = warp - 9;
+    uint32_t base = 0, tiles_before = 0, q_phase = 0;  // (descriptor offsets: 16-byte units)
+    const uint64_t q_desc = smem_desc_sw128(smem_u32(q_s) + s * SLOT_BYTES), k_desc = smem_desc_sw128(smem_u32(ring)),
+                   v_desc = desc_v(smem_u32(ring));
     bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && __all_sync(ALL, mbar_wait(bar, parity, &sh.abort_flag, status));
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      ok = ok && mbar_wait(bar, phase & 1u, &sh.abort_flag, status);
       return ok;
     };
-    auto full = [&](uint32_t at) { return wait(&sh.full[(base + at) % RING], ((base + at) / RING) & 1u); };
-    auto scores = [&](int s, uint32_t at) {  // S = Q K^T of stream s
-      if (lane == 0) {
-        const uint32_t k = ring_u + ((base + at) % RING) * SLOT_BYTES;
+    auto full = [&](uint32_t at) { return wait(&sh.full[(base + at) % RING], (base + at) / RING); };
+    auto scores = [&](int t, int half) {  // S = Q K^T of 64 keys
+      const uint64_t kd = k_desc + ((base + 2 * t) % RING * SLOT_BYTES + half * HALF * 128 >> 4);
+      const uint32_t d = tmem + s * TILE + half * HALF;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint32_t off = (kk >> 2) * (SLOT_BYTES / 2) + (kk & 3) * 32;
-          tc_mma_bf16(tmem + s * TILE, smem_desc_sw128(q_u + s * SLOT_BYTES + off), smem_desc_sw128(k + off), IDESC_QK,
-                      kk > 0);
-        }
-        tc_commit(&sh.s_full[s]);
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint32_t off = ((kk >> 2) * (SLOT_BYTES / 2) + (kk & 3) * 32) >> 4;
+        tc_mma_bf16(d, q_desc + off, kd + off, IDESC_QK, kk > 0);
       }
-      __syncwarp();
+      tc_commit(&sh.s_full[s][half]);
     };
-    bool begun[2] = {false, false};                       // the stream's O holds a product of this segment
-    auto values = [&](int s, uint32_t at) {               // O (+)= P V, the valid blocks only
-      if (lane == 0) {
-        const uint32_t v = ring_u + ((base + at) % RING) * SLOT_BYTES;
-        const uint32_t mask = sh.valid[(base + at) % RING];
-        bool acc = begun[s];
+    bool begun = false;                   // O holds a product of this segment
+    auto values = [&](int t, int half) {  // O (+)= P V, the valid blocks only
+      const uint32_t slot = (base + 2 * t + 1) % RING;
+      const uint64_t vd = v_desc + (slot * SLOT_BYTES + half * 4 * 2048 >> 4);
+      const uint32_t mask = sh.valid[slot] >> (4 * half) & 0xFu;
+      const uint32_t d = tmem + 256 + s * D, a = tmem + s * TILE + half * HALF;
+      if (mask == 0xFu) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma_bf16_ta(d, a + 8 * kk, vd + (kk * 2048 >> 4), IDESC_PV, kk > 0 || begun);
+        begun = true;
+      } else {
+        for (int kk = 0; kk < 4; ++kk) {
           if (!(mask >> kk & 1u)) continue;
-          tc_mma_bf16_ta(tmem + 256 + s * D, tmem + s * TILE + 8 * kk, desc_v(v + kk * 2048), IDESC_PV, acc);
-          acc = true;
+          tc_mma_bf16_ta(d, a + 8 * kk, vd + (kk * 2048 >> 4), IDESC_PV, begun);
+          begun = true;
         }
-        begun[s] = acc;
       }
-      __syncwarp();
+      tc_commit(&sh.o_done[s][half]);
     };
-    auto commit = [&](uint64_t* bar) {
-      if (lane == 0) tc_commit(bar);
-      __syncwarp();
-    };
-    auto release = [&](uint32_t at) { commit(&sh.empty[(base + at) % RING]); };
     while (ok && walk.next(sg)) {
-      const bool pair = sg.nv > TILE;
       const int tiles = sg.t1 - sg.t0;
-      if (!wait(&sh.q_ready[0], q_phase & 1u) || !wait(&sh.q_ready[1], q_phase & 1u)) break;
-      ++q_phase;
-      begun[0] = begun[1] = false;
-      tc_fence_after();
-      if (pair) {
-        if (!full(0)) break;
+      const bool both = sg.nv > TILE;
+      auto release = [&](uint32_t at) {
+        tc_commit(&sh.empty[(base + at) % RING]);
+        if (!both) tc_commit(&sh.empty[(base + at) % RING]);  // (for the query tile that is not there)
+      };
+      if (both || s == 0) {
+        begun = false;
+        if (!wait(&sh.q_ready[s], q_phase++) || !full(0)) break;
+        tc_fence_after();
         scores(0, 0);
-        scores(1, 0);
+        scores(0, 1);
         release(0);
         for (int t = 0; ok && t < tiles; ++t) {
-          if (!full(2 * t + 1)) break;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            if (!wait(&sh.p_ready[s], p_phase[s] & 1u)) break;
-            ++p_phase[s];
-            tc_fence_after();
-            values(s, 2 * t + 1);
-            if (s == 1) release(2 * t + 1);
-            if (t + 1 < tiles) {
-              if (!full(2 * t + 2)) break;
-              scores(s, 2 * t + 2);
-              if (s == 1) release(2 * t + 2);
-            } else {
-              commit(&sh.o_full[s]);
-            }
-          }
-        }
-      } else {
-        for (int s = 0; s < 2 && s < tiles; ++s) {
-          if (!full(s)) break;
-          scores(s, s);
-          release(s);
-        }
-        for (int t = 0; ok && t < tiles; ++t) {
-          const int s = t & 1;
-          const uint32_t v_at = (uint32_t)min(2 * t + 2, 2 * tiles - 1);
-          if (!full(v_at) || !wait(&sh.p_ready[s], p_phase[s] & 1u)) break;
-          ++p_phase[s];
+          if (!full(2 * t + 1) || !wait(&sh.p_ready[s][0], tiles_before + t)) break;
           tc_fence_after();
-          values(s, v_at);
-          release(v_at);
-          if (t + 2 < tiles) {
-            if (!full(2 * t + 3)) break;
-            scores(s, 2 * t + 3);
-            release(2 * t + 3);
-          } else {
-            commit(&sh.o_full[s]);
+          values(t, 0);
+          if (t + 1 < tiles) {
+            if (!full(2 * t + 2)) break;
+            scores(t + 1, 0);
+          }
+          if (!wait(&sh.p_ready[s][1], tiles_before + t)) break;
+          tc_fence_after();
+          values(t, 1);
+          release(2 * t + 1);
+          if (t + 1 < tiles) {
+            scores(t + 1, 1);
+            release(2 * t + 2);
           }
         }
+        tiles_before += tiles;
       }
       base += 2 * tiles;
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -974,37 +1058,26 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS)
     const long long at = ((long long)s * rows.max_rows + row) * nh + head;
     add(parts.own_o, parts.own_m[at], parts.own_l[at], at);
   }
-  const long long work = e.group >= 0 ? parts.group_work[groups.num_groups] : 0;
+  const int work = e.group >= 0 ? parts.group_work[groups.num_groups] : 0;
   if (work > 0) {
     const int g = e.group, blocks = groups.prefix_blocks[g], tiles = key_tiles(blocks);
-    const int vec = (int)(parts.group_vec[g + 1] - parts.group_vec[g]);
+    const int vec_at = parts.group_vec[g], vec = parts.group_vec[g + 1] - vec_at;
     const int v = (parts.entry_at[b] + j) * G + head % G, item = v / 256;
-    const int nv = min(256, vec - 256 * item), u = item_units(nv);
-    const long long from = parts.group_work[g] + h * head_work(vec, blocks) + 2LL * tiles * item;
-    // the CTAs whose range meets the item's units
-    int c = (int)(from * pre_ctas / work);
-    while (c > 0 && cta_bound(work, c, pre_ctas) > from) --c;
-    while (cta_bound(work, c + 1, pre_ctas) <= from) ++c;
-    for (; c < pre_ctas && cta_bound(work, c, pre_ctas) < from + (long long)u * tiles; ++c) {
-      const long long lo = max(cta_bound(work, c, pre_ctas) - from, 0LL), hi = cta_bound(work, c + 1, pre_ctas) - from;
-      const int t0 = (int)((lo + u - 1) / u), t1 = (int)min((long long)tiles, (hi + u - 1) / u);
-      if (t0 >= t1) continue;
-      const long long base = prefix_offset(parts.group_vec[g], nkv, h, vec, item, c);
-      if (nv > TILE) {
-        const long long at = base + v - 256 * item;
-        add(parts.pre_o, parts.pre_m[at], parts.pre_l[at], at);
-      } else {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const long long at = base + s * nv + v - 256 * item;
-          add(parts.pre_o, parts.pre_m[at], parts.pre_l[at], at);
-        }
-      }
+    const int nv = min(256, vec - 256 * item), u = item_units(nv), per = (work + pre_ctas - 1) / pre_ctas;
+    // the CTAs whose units meet the item's
+    const int from = parts.group_work[g] + h * head_work(vec, blocks) + 4 * tiles * item, to = from + u * tiles;
+    for (int c = from / per; c * per < to; ++c) {
+      // (a CTA does the key tiles whose first unit is among its own)
+      const int first = max(c * per - from, 0) + u - 1, last = (c + 1) * per - from + u - 1;
+      if (first / u >= min(tiles, last / u)) continue;
+      const long long base = prefix_offset(vec_at, nkv, h, vec, item, c) + v - 256 * item;
+      add(parts.pre_o, parts.pre_m[base], parts.pre_l[base], base);
     }
   }
   // (l is 0 only for a row that sees no key; NaN stays NaN)
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
+  const float inv = 1.f / l;
+  __nv_bfloat162 y[2] = {__floats2bfloat162_rn(l == 0.f ? 0.f : o.x * inv, l == 0.f ? 0.f : o.y * inv),
+                         __floats2bfloat162_rn(l == 0.f ? 0.f : o.z * inv, l == 0.f ? 0.f : o.w * inv)};
   *reinterpret_cast<uint2*>(out + ((long long)row * nh + head) * D + 4 * lane) = *reinterpret_cast<uint2*>(y);
 }
 
@@ -1041,12 +1114,17 @@ int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const vo
   const int splits = own_splits(rows.num_seqs, nkv, tiles, rows.max_context, sms);
   const Layout l = layout_of(rows.max_rows, rows.num_seqs, groups.num_groups, nh, splits, sms);
   if (ws_bytes < l.total) return NE_ERR_WORKSPACE;
-  if ((long long)tiles * splits > 65535 || nkv > 65535) return NE_ERR_UNSUPPORTED;
+  // grid limits; rows of an entry in 20 bits, and units of work in 31
+  if ((long long)tiles * splits > 65535 || nkv > 65535 || rows.max_q_len >= (1 << 20) ||
+      (long long)rows.max_rows * nh >= (1 << 29) ||
+      ((long long)rows.max_rows * nh / TILE + 2LL * groups.num_groups * nkv + 2) * (groups.max_prefix_blocks / 8 + 1) >=
+          (1 << 29))
+    return NE_ERR_UNSUPPORTED;
   if (kv_int8 || groups.max_prefix_blocks == 0) groups.num_groups = 0;
   auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
   const Parts parts{f(l.own_o), f(l.own_m), f(l.own_l), f(l.pre_o), f(l.pre_m), f(l.pre_l),
-                    reinterpret_cast<int32_t*>(ws + l.entry_at), reinterpret_cast<long long*>(ws + l.group_work),
-                    reinterpret_cast<long long*>(ws + l.group_vec), splits};
+                    reinterpret_cast<int32_t*>(ws + l.entry_at), reinterpret_cast<int32_t*>(ws + l.group_work),
+                    reinterpret_cast<int32_t*>(ws + l.group_vec), splits};
   static bool own_done[2][64] = {}, pre_done[64] = {};
   auto own = kv_int8 ? own_tokens_kernel<true> : own_tokens_kernel<false>;
   if (!allow_smem(own, OWN_SMEM, own_done[kv_int8 ? 1 : 0])) return NE_ERR_CUDA;

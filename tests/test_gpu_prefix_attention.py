@@ -198,6 +198,30 @@ def test_later_rows_values_do_not_reach_earlier_rows(ops) -> None:
     assert_close(got, c, rows=clean)
 
 
+@pytest.mark.parametrize("where", ["query", "prefix key", "own key", "prefix value", "own value"])
+def test_nan_that_a_row_sees_reaches_it(ops, where) -> None:
+    """NaN in a query, or in a key or value its row sees, gives NaN there; every other row and head
+    stays as near the definition as it is without (a warp that meets a NaN takes all its rows' powers
+    of two on the special-function unit, so not bit for bit)."""
+    c = make_case(19, 16, 8, [5] * 6, [272], [0] * 6, [9, 30, 1, 0, 70, 3])
+    hit = torch.zeros(30, 16, dtype=torch.bool, device=c["q"].device)
+    if where == "query":
+        c["q"][7, 3, 60] = float("nan")
+        hit[7, 3] = True
+    else:
+        entry, at = (2, 100) if where.startswith("prefix") else (4, 300)
+        slot = int(c["table"][entry][at // BLOCK]) * BLOCK + at % BLOCK
+        c["k" if "key" in where else "v"][slot, 5, 7] = float("nan")
+        rows = torch.arange(30, device=hit.device)
+        seen = torch.ones_like(rows, dtype=torch.bool) if entry == 2 else (rows >= 20) & (rows < 25) & (c["positions"] >= at)
+        hit[seen, 10:12] = True
+    got, status = call(ops, c)
+    assert int(status.item()) == 0
+    bad = torch.isnan(got).any(-1)
+    assert torch.equal(bad, hit), (int(bad.sum()), int(hit.sum()))
+    assert_close(got, c, rows=~hit)
+
+
 def test_rows_of_no_entry_stay_as_they_were(ops) -> None:
     c = make_case(9, 16, 8, [2, 3], [32], [0, 0], [5, 6])
     extra = torch.zeros(4, 16, D, dtype=torch.bfloat16, device=c["q"].device)
