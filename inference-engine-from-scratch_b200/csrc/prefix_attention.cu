@@ -1,12 +1,15 @@
 // Paged attention for a batch whose sequences share prompt prefixes (include/nespec.h,
 // ne_prefix_attention), in three launches:
 //
-// * own_tokens_kernel: every entry against the tokens that are its own (all of them for an entry
-//   without a group), 16 query vectors a tile on mma.sync, one CTA per (entry, KV head, tile, split).
 // * prefix_kernel: every group's query vectors, gathered over its entries, against its prefix:
 //   tcgen05 tiles of 128 vectors x 128 keys, persistent CTAs that divide all prefixes' tiles evenly.
-// * join_kernel: o = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m) over an entry's parts i, each an
-//   unnormalised sum O_i of values, its sum of weights l_i and the (log2) reference m_i of both.
+// * own_tokens_kernel: every entry against the tokens that are its own (all of them for an entry
+//   without a group), 16 query vectors a tile on mma.sync, one CTA per (entry, KV head, tiles). It
+//   starts on the SMs that prefix_kernel's first CTAs leave.
+// * join_kernel: o = sum O_i 2^(m_i - m) / sum l_i 2^(m_i - m) over a vector's parts i, each an
+//   unnormalised sum O_i of values, its sum of weights l_i and the (log2) reference m_i of both. (The
+//   join inside own_tokens_kernel was measured and is slower: a CTA's few warps then wait for every
+//   vector's parts in turn, 11,000 to 30,000 cycles.)
 #include <algorithm>
 
 #include "attention.cuh"
@@ -32,7 +35,7 @@ struct Parts {
   int32_t* entry_at;      // [num_seqs] the entry's first row among its group's
   int32_t* group_work;    // [num_groups + 1] units of work before group g
   int32_t* group_vec;     // [num_groups + 1] vectors of one KV head before group g
-  int splits;
+  int splits, pre_ctas;
 };
 
 constexpr size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -76,8 +79,8 @@ struct Entry {
 // out; a group is taken only if the entry's first row (its positions ascend) sees its whole prefix.
 __device__ __forceinline__ Entry entry_of(const ne_rows& rows, const ne_prefix_groups& groups, int b, int* status) {
   Entry e{rows.q_len[b], rows.q_start[b], -1};
-  if (e.rows <= 0) return Entry{0, 0, -1};
   const int g = groups.num_groups > 0 ? groups.entry_group[b] : -1;
+  if (e.rows <= 0) return Entry{0, 0, -1};
   if (e.rows > rows.max_q_len || e.start < 0 || e.start > rows.max_rows - e.rows) {
     report(status, NE_DEV_BAD_SLOT);
     return Entry{0, 0, -1};
@@ -99,6 +102,86 @@ __device__ __forceinline__ float max2(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
+}
+
+// ---------------------------------------------------------------- prefixes: the division of the work
+// A group's vectors of one KV head are cut into items of up to 256: one or two query tiles, which share
+// every tile of 128 keys. A key tile costs an item 3 units of work with one query tile and 4 with two
+// (measured: about 1,900 and 2,500 cycles). The units of all (group, head, item) in turn are divided
+// evenly over the CTAs: CTA c does the key tiles that start in its ceil(W / CTAs) units from
+// c ceil(W / CTAs) on.
+__device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 7) / 8; }
+__device__ __forceinline__ int item_units(int vec) { return vec > TILE ? 4 : 3; }
+// units of one KV head
+__device__ __forceinline__ int head_work(int vec, int blocks) {
+  const int rest = vec % 256;
+  return key_tiles(blocks) * (4 * (vec / 256) + (rest ? item_units(rest) : 0));
+}
+// Where the part of (CTA c, item) lies: behind the vectors of the items before it and 256 for each CTA
+// before it; a part has at most 256, so that consecutive ones do not overlap.
+__device__ __forceinline__ long long prefix_offset(long long vec_at, int nkv, int h, int vec, int item, int cta) {
+  return vec_at * nkv + (long long)h * vec + 256LL * item + 256LL * cta;
+}
+
+// ---------------------------------------------------------------- the join of a vector's parts
+// A warp's running sums of one query vector: four dimensions a lane.
+struct Sums {
+  float m = -INFINITY, l = 0.f;
+  float4 o = {0.f, 0.f, 0.f, 0.f};
+
+  // Up to 32 parts, lane p's at position ``at`` of (po, m, l); m -inf: an empty part, whose sums were
+  // never written. Every lane reads its part's m and l at once, then all lanes each part's values.
+  __device__ __forceinline__ void add(const float* po, float pm, float pl, long long at, int count) {
+    const int lane = threadIdx.x & 31;
+    float top = pm;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = max2(top, __shfl_xor_sync(ALL, top, x));
+    const float mn = max2(m, top);
+    if (mn == NEG_INF) return;
+    const float keep = m == NEG_INF ? 0.f : exp2f(m - mn), f = pm == NEG_INF ? 0.f : exp2f(pm - mn);
+    float sum = pm == NEG_INF ? 0.f : f * pl;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(ALL, sum, x);
+    l = l * keep + sum;
+    m = mn;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll 4
+    for (int p = 0; p < count; ++p) {
+      const float fp = __shfl_sync(ALL, f, p);
+      const long long ap = __shfl_sync(ALL, at, p);
+      if (fp == 0.f) continue;
+      const float4 y = *reinterpret_cast<const float4*>(po + ap * D + 4 * lane);
+      o = make_float4(o.x + fp * y.x, o.y + fp * y.y, o.z + fp * y.z, o.w + fp * y.w);
+    }
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* out) const {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // (l is 0 only for a row that sees no key; NaN stays NaN)
+    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(l == 0.f ? 0.f : o.x * inv, l == 0.f ? 0.f : o.y * inv),
+                           __floats2bfloat162_rn(l == 0.f ? 0.f : o.z * inv, l == 0.f ? 0.f : o.w * inv)};
+    *reinterpret_cast<uint2*>(out + 4 * (threadIdx.x & 31)) = *reinterpret_cast<uint2*>(y);
+  }
+};
+
+// Adds the prefix parts of query head ``h * G + hq`` of row ``j`` of entry b, whose prefix has ``blocks``.
+__device__ __forceinline__ void add_prefix(Sums& sums, const Parts& parts, int num_groups, int g, int blocks, int b,
+                                           int j, int h, int hq, int G, int nkv) {
+  const int work = parts.group_work[num_groups], tiles = key_tiles(blocks);
+  const int vec_at = parts.group_vec[g], vec = parts.group_vec[g + 1] - vec_at;
+  const int v = (parts.entry_at[b] + j) * G + hq, item = v / 256;
+  if (work == 0) return;
+  const int nv = min(256, vec - 256 * item), u = item_units(nv), per = (work + parts.pre_ctas - 1) / parts.pre_ctas;
+  // the CTAs whose units meet the item's
+  const int from = parts.group_work[g] + h * head_work(vec, blocks) + 4 * tiles * item, to = from + u * tiles;
+  const long long at0 = prefix_offset(vec_at, nkv, h, vec, item, 0) + v - 256 * item;
+  for (int c0 = from / per; c0 * per < to; c0 += 32) {
+    const int c = c0 + (threadIdx.x & 31);
+    const int count = min(32, (to - c0 * per + per - 1) / per);
+    // (a CTA does the key tiles whose first unit is among its own)
+    const int first = max(c * per - from, 0) + u - 1, last = (c + 1) * per - from + u - 1;
+    const bool has = c * per < to && first / u < min(tiles, last / u);
+    const long long at = at0 + 256LL * c;
+    sums.add(parts.pre_o, has ? parts.pre_m[at] : NEG_INF, has ? parts.pre_l[at] : 0.f, at, count);
+  }
 }
 
 // ---------------------------------------------------------------- own tokens
@@ -238,28 +321,37 @@ __device__ __forceinline__ void own_block(TileState& ts, uint32_t k_s, uint32_t 
   }
 }
 
-constexpr int OWN_WARPS = 4;
-constexpr size_t OWN_SMEM = BLOCK_BYTES + 128 + (size_t)OWN_WARPS * 4 * BLOCK_BYTES;
-static_assert((OWN_WARPS * 16 * D + 2 * OWN_WARPS * 16) * 4 <= OWN_WARPS * 4 * BLOCK_BYTES, "merge area");
+// NW groups of NT warps: group w takes every NW-th block of the split into two cp.async stages of its
+// own, its warp t serves query tile t, and the groups merge their sums at the end.
+template <int NW, int NT>
+constexpr size_t own_smem() {
+  return (size_t)NT * BLOCK_BYTES + 128 + (size_t)NW * 4 * BLOCK_BYTES;
+}
+static_assert((2 * 4 * 16 * D + 2 * 2 * 4 * 16) * 4 <= 4 * 4 * BLOCK_BYTES, "merge area");
 
-// The four warps take every fourth block of the split, each with two cp.async stages of its own, and
-// merge their sums through shared memory. Bound by memory: each block is read once per tile.
-template <bool INT8>
-__global__ void __launch_bounds__(32 * OWN_WARPS, 3)
+// Bound by memory: each block is read once per CTA, a CTA's first loads go out before its query tile.
+template <bool INT8, int NW, int NT>
+__global__ void __launch_bounds__(32 * NW * NT, NT == 2 ? 2 : NW == 8 ? 1 : NW == 4 ? 3 : 5)
     own_tokens_kernel(const __nv_bfloat16* __restrict__ q, const void* __restrict__ kc, const void* __restrict__ vc,
                       const __nv_bfloat16* __restrict__ ks, const __nv_bfloat16* __restrict__ vs, ne_rows rows,
-                      ne_prefix_groups groups, int nh, int nkv, long long num_cache_slots, Parts parts, int tiles,
-                      int* status) {
-  pdl_prologue();
+                      ne_prefix_groups groups, int nh, int nkv, long long num_cache_slots, Parts parts, int chunks,
+                      int late_wait, int* status) {
+  // behind prefix_kernel, whose CTAs let this launch start only after they waited for the launch
+  // before them, no input is still being written; the wait for that kernel itself comes at the end
+  if (!late_wait) pdl_wait();
+  pdl_trigger();
   extern __shared__ __align__(16) uint8_t smem[];
-  const int b = blockIdx.x, h = blockIdx.y, tile = blockIdx.z % tiles, split = blockIdx.z / tiles;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Entry e = entry_of(rows, groups, b, tid == 0 && tile == 0 && h == 0 && split == 0 ? status : nullptr);
+  const int b = blockIdx.x, h = blockIdx.y, chunk = blockIdx.z % chunks, split = blockIdx.z / chunks;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp % NW, tile = warp / NW;
+  const Entry e = entry_of(rows, groups, b, tid == 0 && chunk == 0 && h == 0 && split == 0 ? status : nullptr);
   Ctx c{};
   c.G = nh / nkv;
   c.nvec = e.rows * c.G;
-  const int v_base = 16 * tile;
-  if (v_base >= c.nvec) return;
+  const int v_base = 16 * NT * chunk;
+  if (v_base >= c.nvec) {
+    pdl_wait();
+    return;
+  }
   c.q = q;
   c.kc = kc;
   c.vc = vc;
@@ -273,20 +365,24 @@ __global__ void __launch_bounds__(32 * OWN_WARPS, 3)
   c.num_cache_slots = num_cache_slots;
   c.status = status;
   uint8_t* q_s = smem;
-  int* spos = reinterpret_cast<int*>(smem + BLOCK_BYTES);
-  uint8_t* buf = smem + BLOCK_BYTES + 128;
-  const uint32_t wbuf = smem_u32(buf) + warp * 4 * BLOCK_BYTES;
-  const int v_last = min(c.nvec, v_base + 16) - 1;
-  const int last = rows.positions[c.r0 + v_last / c.G];  // the tile's last row sees the most
+  int* spos = reinterpret_cast<int*>(smem + NT * BLOCK_BYTES);
+  uint8_t* buf = smem + NT * BLOCK_BYTES + 128;
+  const uint32_t wbuf = smem_u32(buf) + group * 4 * BLOCK_BYTES;
+  const int v_end = min(c.nvec, v_base + 16 * NT);
+  const int last = rows.positions[c.r0 + (v_end - 1) / c.G];  // the chunk's last row sees the most
   const int nblk = last >= 0 ? last / 16 + 1 : 0;
   const int kb_first = e.group >= 0 ? groups.prefix_blocks[e.group] : 0;
   const int n = max(0, nblk - kb_first), per_split = (n + parts.splits - 1) / parts.splits;
   const int kb0 = kb_first + split * per_split, kb1 = min(nblk, kb0 + per_split);
   const int stride = rows.block_table_stride;
-  // this warp's blocks kb0 + warp + 4 j; the table entries of 32 of them in the lanes of a register
-  const int count = kb0 + warp < kb1 ? (kb1 - kb0 - warp + OWN_WARPS - 1) / OWN_WARPS : 0;
+  auto group_sync = [&] {
+    if (NT == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * NT) : "memory");
+  };
+  // this group's blocks kb0 + group + NW j; the table entries of 32 of them in the lanes of a register
+  const int count = kb0 + group < kb1 ? (kb1 - kb0 - group + NW - 1) / NW : 0;
   auto table_chunk = [&](int j0) -> int {
-    const int kb = kb0 + warp + OWN_WARPS * (j0 + lane);
+    const int kb = kb0 + group + NW * (j0 + lane);
     return kb < kb1 && kb < stride ? c.table[kb] : -1;
   };
   int tbl = table_chunk(0);
@@ -298,101 +394,99 @@ __global__ void __launch_bounds__(32 * OWN_WARPS, 3)
   auto stage = [&](int j, long long blk) {
     if (blk >= 0) {
       if (INT8) {
-        stage_raw_int8(c, blk, wbuf + (j & 1) * 4096, lane);
+        if (tile == 0) stage_raw_int8(c, blk, wbuf + (j & 1) * 4096, lane);
         next_scales = load_scales_int8(c, blk, lane);
       } else {
         const uint32_t at = wbuf + (j & 1) * 2 * BLOCK_BYTES;
-        stage_block<false>(c, blk, at, at + BLOCK_BYTES, lane, 32);
+        stage_block<false>(c, blk, at, at + BLOCK_BYTES, lane + 32 * tile, 32 * NT);
       }
     }
     cp_commit();
   };
   long long blk = count > 0 ? block_at(0) : -1;
   stage(0, blk);
-  if (tid < 16) spos[tid] = v_base + tid < c.nvec ? rows.positions[c.r0 + (v_base + tid) / c.G] : -1;
-  load_q_tile(c, v_base, q_s, tid, 32 * OWN_WARPS);
+  if (tid < 16 * NT) spos[tid] = v_base + tid < c.nvec ? rows.positions[c.r0 + (v_base + tid) / c.G] : -1;
+  {  // the query tiles: 16 chunks of 16 bytes a vector, every load issued before the first store
+    constexpr int PER = 256 * NT / (32 * NW * NT);
+    uint4 x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int v = v_base + ((tid + i * 32 * NW * NT) >> 4), ch = tid & 15;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (v < c.nvec)
+        x[i] = *reinterpret_cast<const uint4*>(c.q + ((long long)(c.r0 + v / c.G) * c.nh + c.h * c.G + v % c.G) * D + ch * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      *reinterpret_cast<uint4*>(q_s + ((tid + i * 32 * NW * NT) >> 4) * ROW_BYTES + (tid & 15) * 16) = x[i];
+  }
   __syncthreads();
   TileState ts;
-  tile_init(ts, smem_u32(q_s), spos, lane);
+  tile_init(ts, smem_u32(q_s) + tile * BLOCK_BYTES, spos + 16 * tile, lane);
   for (int j = 0; j < count; ++j) {
     scales = next_scales;
     const long long next = j + 1 < count ? block_at(j + 1) : -1;
     stage(j + 1, next);
     cp_wait<1>();
-    __syncwarp();
+    group_sync();
     if (blk >= 0) {
-      const int kb = kb0 + warp + OWN_WARPS * j;
-      if (INT8) {
+      const int kb = kb0 + group + NW * j;
+      if (INT8) {  // (scale 1: the integers, exact in bf16; two warps convert a half each)
         const uint32_t raw = wbuf + (j & 1) * 4096, kv = wbuf + 8192;
-        convert_raw_int8(raw, kv, kv + BLOCK_BYTES, 0x3F80u, lane);  // (scale 1: the integers, exact in bf16)
-        __syncwarp();
+        if (tile == 0) convert_half_int8(raw, kv, 0x3F80u, 0, lane);
+        if (tile == NT - 1) convert_half_int8(raw + 2048, kv + BLOCK_BYTES, 0x3F80u, 16, lane);
+        group_sync();
         own_block<true>(ts, kv, kv + BLOCK_BYTES, kb, scales, lane);
       } else {
         const uint32_t at = wbuf + (j & 1) * 2 * BLOCK_BYTES;
         own_block<false>(ts, at, at + BLOCK_BYTES, kb, 0u, lane);
       }
     }
-    __syncwarp();
+    group_sync();
     blk = next;
   }
   cp_wait<0>();
   __syncthreads();
-  float* mo = reinterpret_cast<float*>(buf);  // [warps][16][128]
-  float* mm = mo + OWN_WARPS * 16 * D;        // [warps][16]
-  float* ml = mm + OWN_WARPS * 16;
+  float* mo = reinterpret_cast<float*>(buf);  // [NT][NW][16][128]
+  float* mm = mo + NT * NW * 16 * D;          // [NT][NW][16]
+  float* ml = mm + NT * NW * 16;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int row = (lane >> 2) + 8 * r;
+    const int at = warp * 16 + (lane >> 2) + 8 * r;
 #pragma unroll
     for (int t = 0; t < 16; ++t)
-      *reinterpret_cast<float2*>(&mo[(warp * 16 + row) * D + 8 * t + 2 * (lane & 3)]) =
-          make_float2(ts.o[t][2 * r], ts.o[t][2 * r + 1]);
+      *reinterpret_cast<float2*>(&mo[at * D + 8 * t + 2 * (lane & 3)]) = make_float2(ts.o[t][2 * r], ts.o[t][2 * r + 1]);
     if ((lane & 3) == 0) {
-      mm[warp * 16 + row] = ts.m[r];
-      ml[warp * 16 + row] = ts.l[r];
+      mm[at] = ts.m[r];
+      ml[at] = ts.l[r];
     }
   }
   __syncthreads();
-  for (int v = 0; v < v_last - v_base + 1; ++v) {
-    float m = NEG_INF, l = 0.f, o = 0.f;
+  // a warp per vector: four dimensions a lane
+  for (int x = warp; x < v_end - v_base; x += NW * NT) {
+    const int at = (x >> 4) * NW * 16 + (x & 15);
+    float m = mm[at];
 #pragma unroll
-    for (int w = 0; w < OWN_WARPS; ++w) m = fmaxf(m, mm[w * 16 + v]);
+    for (int w = 1; w < NW; ++w) m = max2(m, mm[at + 16 * w]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < OWN_WARPS; ++w) {
-      const float mw = mm[w * 16 + v];
-      const float f = mw == NEG_INF ? 0.f : exp2f(mw - m);
-      if (f != 0.f) {
-        l += ml[w * 16 + v] * f;
-        o += mo[(w * 16 + v) * D + tid] * f;
-      }
+    for (int w = 0; w < NW; ++w) {
+      const float mw = mm[at + 16 * w], f = mw == NEG_INF ? 0.f : exp2f(mw - m);
+      const float4 y = *reinterpret_cast<const float4*>(&mo[(at + 16 * w) * D + 4 * lane]);
+      if (mw == NEG_INF) continue;  // (a group without blocks)
+      l += f * ml[at + 16 * w];
+      o = make_float4(o.x + f * y.x, o.y + f * y.y, o.z + f * y.z, o.w + f * y.w);
     }
-    const int row = c.r0 + (v_base + v) / c.G, head = h * c.G + (v_base + v) % c.G;
-    const long long at = ((long long)split * rows.max_rows + row) * nh + head;
-    parts.own_o[at * D + tid] = o;
-    if (tid == 0) {
-      parts.own_m[at] = m;
-      parts.own_l[at] = l;
+    const int row = c.r0 + (v_base + x) / c.G, head = h * c.G + (v_base + x) % c.G;
+    const long long to = ((long long)split * rows.max_rows + row) * nh + head;
+    *reinterpret_cast<float4*>(parts.own_o + to * D + 4 * lane) = o;
+    if (lane == 0) {
+      parts.own_m[to] = m;
+      parts.own_l[to] = l;
     }
   }
-}
-
-// ---------------------------------------------------------------- prefixes: the division of the work
-// A group's vectors of one KV head are cut into items of up to 256: one or two query tiles, which share
-// every tile of 128 keys. A key tile costs an item 3 units of work with one query tile and 4 with two
-// (measured: about 1,900 and 2,500 cycles). The units of all (group, head, item) in turn are divided
-// evenly over the CTAs: CTA c does the key tiles that start in its ceil(W / CTAs) units from
-// c ceil(W / CTAs) on.
-__device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 7) / 8; }
-__device__ __forceinline__ int item_units(int vec) { return vec > TILE ? 4 : 3; }
-// units of one KV head
-__device__ __forceinline__ int head_work(int vec, int blocks) {
-  const int rest = vec % 256;
-  return key_tiles(blocks) * (4 * (vec / 256) + (rest ? item_units(rest) : 0));
-}
-// Where the part of (CTA c, item) lies: behind the vectors of the items before it and 256 for each CTA
-// before it; a part has at most 256, so that consecutive ones do not overlap.
-__device__ __forceinline__ long long prefix_offset(long long vec_at, int nkv, int h, int vec, int item, int cta) {
-  return vec_at * nkv + (long long)h * vec + 256LL * item + 256LL * cta;
+  pdl_wait();  // (no launch behind this one sees it complete before prefix_kernel is)
 }
 
 // ---------------------------------------------------------------- prefixes: the tensor-core kernel
@@ -600,7 +694,8 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                   const __nv_bfloat16* __restrict__ q, ne_rows rows, ne_prefix_groups groups, int nh, int nkv,
                   long long num_cache_slots, Parts parts, int* status) {
-  pdl_prologue();
+  pdl_wait();
+  pdl_trigger();  // (after the wait: own_tokens_kernel relies on it)
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* q_s = smem;                              // [2 streams] query tiles
@@ -1033,52 +1128,23 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
 // ---------------------------------------------------------------- the join
 constexpr int JOIN_WARPS = 8;
 
-// A warp per vector: four dimensions a lane.
+// A warp per vector. Bound by latency: three loads in a row behind the wait (where the parts are,
+// their sums of weights, their values), the inputs before it.
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
-    join_kernel(__nv_bfloat16* __restrict__ out, ne_rows rows, ne_prefix_groups groups, int nh, int nkv, Parts parts,
-                int pre_ctas) {
-  pdl_prologue();
+    join_kernel(__nv_bfloat16* __restrict__ out, ne_rows rows, ne_prefix_groups groups, int nh, int nkv, Parts parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
   const Entry e = entry_of(rows, groups, b, nullptr);
-  const int x = blockIdx.y * JOIN_WARPS + warp;
+  const int x = blockIdx.y * JOIN_WARPS + warp, blocks = e.group >= 0 ? groups.prefix_blocks[e.group] : 0;
+  pdl_prologue();
   if (x >= e.rows * nh) return;
-  const int j = x / nh, head = x % nh, G = nh / nkv, h = head / G;
-  const int row = e.start + j;
-  float m = NEG_INF, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float* po, float pm, float pl, long long at) {
-    if (pm == NEG_INF) return;  // (an empty part: its sums were never written)
-    const float mn = fmaxf(m, pm), f = m == NEG_INF ? 0.f : exp2f(m - mn), g = exp2f(pm - mn);
-    const float4 y = *reinterpret_cast<const float4*>(po + at * D + 4 * lane);
-    m = mn;
-    l = l * f + pl * g;
-    o = make_float4(o.x * f + y.x * g, o.y * f + y.y * g, o.z * f + y.z * g, o.w * f + y.w * g);
-  };
-  for (int s = 0; s < parts.splits; ++s) {
-    const long long at = ((long long)s * rows.max_rows + row) * nh + head;
-    add(parts.own_o, parts.own_m[at], parts.own_l[at], at);
-  }
-  const int work = e.group >= 0 ? parts.group_work[groups.num_groups] : 0;
-  if (work > 0) {
-    const int g = e.group, blocks = groups.prefix_blocks[g], tiles = key_tiles(blocks);
-    const int vec_at = parts.group_vec[g], vec = parts.group_vec[g + 1] - vec_at;
-    const int v = (parts.entry_at[b] + j) * G + head % G, item = v / 256;
-    const int nv = min(256, vec - 256 * item), u = item_units(nv), per = (work + pre_ctas - 1) / pre_ctas;
-    // the CTAs whose units meet the item's
-    const int from = parts.group_work[g] + h * head_work(vec, blocks) + 4 * tiles * item, to = from + u * tiles;
-    for (int c = from / per; c * per < to; ++c) {
-      // (a CTA does the key tiles whose first unit is among its own)
-      const int first = max(c * per - from, 0) + u - 1, last = (c + 1) * per - from + u - 1;
-      if (first / u >= min(tiles, last / u)) continue;
-      const long long base = prefix_offset(vec_at, nkv, h, vec, item, c) + v - 256 * item;
-      add(parts.pre_o, parts.pre_m[base], parts.pre_l[base], base);
-    }
-  }
-  // (l is 0 only for a row that sees no key; NaN stays NaN)
-  const float inv = 1.f / l;
-  __nv_bfloat162 y[2] = {__floats2bfloat162_rn(l == 0.f ? 0.f : o.x * inv, l == 0.f ? 0.f : o.y * inv),
-                         __floats2bfloat162_rn(l == 0.f ? 0.f : o.z * inv, l == 0.f ? 0.f : o.w * inv)};
-  *reinterpret_cast<uint2*>(out + ((long long)row * nh + head) * D + 4 * lane) = *reinterpret_cast<uint2*>(y);
+  const int j = x / nh, head = x % nh, G = nh / nkv;
+  const long long at = ((long long)lane * rows.max_rows + e.start + j) * nh + head;
+  const bool has = lane < parts.splits;  // (at most 16 splits)
+  Sums sums;
+  sums.add(parts.own_o, has ? parts.own_m[at] : NEG_INF, has ? parts.own_l[at] : 0.f, at, parts.splits);
+  if (e.group >= 0)
+    add_prefix(sums, parts, groups.num_groups, e.group, blocks, b, j, head / G, head % G, G, nkv);
+  sums.store(out + ((long long)(e.start + j) * nh + head) * D);
 }
 
 int device_sms() {
@@ -1087,10 +1153,13 @@ int device_sms() {
   return sms;
 }
 
+// Chunks of an entry's query vectors: one of up to 32, or as many of 32 as it takes.
+int own_chunks(int max_q_len, int G) { return (int)(((long long)max_q_len * G + 31) / 32); }
+
 // Splits of the entries' own tokens: one, unless the launch leaves most SMs idle and contexts are long
 // (32 blocks a split at least, as attention_plan_splits).
-int own_splits(int num_seqs, int nkv, int tiles, int max_context, int sms) {
-  const long long ctas = (long long)num_seqs * nkv * tiles;
+int own_splits(int num_seqs, int nkv, int chunks, int max_context, int sms) {
+  const long long ctas = (long long)num_seqs * nkv * chunks;
   long long splits = (2LL * sms + ctas - 1) / ctas;
   splits = std::min<long long>(splits, max_context / 16 / 32);
   return (int)std::max<long long>(1, std::min<long long>(splits, 16));
@@ -1110,27 +1179,22 @@ int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const vo
                             const ne_rows& rows, ne_prefix_groups groups, int nh, int nkv, long long slots,
                             uint8_t* ws, size_t ws_bytes, int* status, cudaStream_t stream) {
   const int sms = device_sms(), G = nh / nkv;
-  const int tiles = (int)(((long long)rows.max_q_len * G + 15) / 16);
-  const int splits = own_splits(rows.num_seqs, nkv, tiles, rows.max_context, sms);
+  const int chunks = own_chunks(rows.max_q_len, G);
+  const int splits = own_splits(rows.num_seqs, nkv, chunks, rows.max_context, sms);
   const Layout l = layout_of(rows.max_rows, rows.num_seqs, groups.num_groups, nh, splits, sms);
   if (ws_bytes < l.total) return NE_ERR_WORKSPACE;
   // grid limits; rows of an entry in 20 bits, and units of work in 31
-  if ((long long)tiles * splits > 65535 || nkv > 65535 || rows.max_q_len >= (1 << 20) ||
+  if ((long long)chunks * splits > 65535 || nkv > 65535 || rows.max_q_len >= (1 << 20) ||
       (long long)rows.max_rows * nh >= (1 << 29) ||
       ((long long)rows.max_rows * nh / TILE + 2LL * groups.num_groups * nkv + 2) * (groups.max_prefix_blocks / 8 + 1) >=
-          (1 << 29))
+          (1 << 28))
     return NE_ERR_UNSUPPORTED;
   if (kv_int8 || groups.max_prefix_blocks == 0) groups.num_groups = 0;
   auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
   const Parts parts{f(l.own_o), f(l.own_m), f(l.own_l), f(l.pre_o), f(l.pre_m), f(l.pre_l),
                     reinterpret_cast<int32_t*>(ws + l.entry_at), reinterpret_cast<int32_t*>(ws + l.group_work),
-                    reinterpret_cast<int32_t*>(ws + l.group_vec), splits};
-  static bool own_done[2][64] = {}, pre_done[64] = {};
-  auto own = kv_int8 ? own_tokens_kernel<true> : own_tokens_kernel<false>;
-  if (!allow_smem(own, OWN_SMEM, own_done[kv_int8 ? 1 : 0])) return NE_ERR_CUDA;
-  if (launch_kernel(own, dim3(rows.num_seqs, nkv, tiles * splits), dim3(32 * OWN_WARPS), OWN_SMEM, stream, q, k_cache,
-                    v_cache, k_scale, v_scale, rows, groups, nh, nkv, slots, parts, tiles, status) != cudaSuccess)
-    return NE_ERR_CUDA;
+                    reinterpret_cast<int32_t*>(ws + l.group_vec), splits, sms};
+  static bool pre_done[64] = {};
   if (groups.num_groups > 0) {
     CUtensorMap kmap, vmap;
     if (!make_tmap_kv(&kmap, k_cache, nkv, slots) || !make_tmap_kv(&vmap, v_cache, nkv, slots)) return NE_ERR_CUDA;
@@ -1139,9 +1203,38 @@ int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const vo
                       nkv, slots, parts, status) != cudaSuccess)
       return NE_ERR_CUDA;
   }
+  // one query tile of up to 16 vectors: eight warps where that leaves at most a CTA an SM, two where
+  // there are many short waves anyway (measured, the whole call: 512 CTAs of 10 blocks 41.3 us with two
+  // warps, 38.3 with four; 2048 CTAs of 7 blocks 89.8 and 97.9); two tiles (up to 32, or chunks of 32):
+  // four pairs of warps
+  const long long ctas = (long long)rows.num_seqs * nkv * chunks * splits;
+  const bool one = (long long)rows.max_q_len * G <= 16;
+  const int late = groups.num_groups > 0 ? 1 : 0;
+  auto launch = [&](auto kernel, size_t smem, int threads, bool (&done)[64]) {
+    if (!allow_smem(kernel, smem, done)) return (int)NE_ERR_CUDA;
+    return launch_kernel(kernel, dim3(rows.num_seqs, nkv, chunks * splits), dim3(threads), smem, stream, q, k_cache,
+                         v_cache, k_scale, v_scale, rows, groups, nh, nkv, slots, parts, chunks, late,
+                         status) == cudaSuccess ? (int)NE_OK : (int)NE_ERR_CUDA;
+  };
+  static bool done[8][64] = {};
+  int rc;
+  if (!one) {
+    rc = kv_int8 ? launch(own_tokens_kernel<true, 4, 2>, own_smem<4, 2>(), 256, done[0])
+                 : launch(own_tokens_kernel<false, 4, 2>, own_smem<4, 2>(), 256, done[1]);
+  } else if (ctas <= sms) {
+    rc = kv_int8 ? launch(own_tokens_kernel<true, 8, 1>, own_smem<8, 1>(), 256, done[2])
+                 : launch(own_tokens_kernel<false, 8, 1>, own_smem<8, 1>(), 256, done[3]);
+  } else if (ctas <= 6LL * sms) {
+    rc = kv_int8 ? launch(own_tokens_kernel<true, 4, 1>, own_smem<4, 1>(), 128, done[4])
+                 : launch(own_tokens_kernel<false, 4, 1>, own_smem<4, 1>(), 128, done[5]);
+  } else {
+    rc = kv_int8 ? launch(own_tokens_kernel<true, 2, 1>, own_smem<2, 1>(), 64, done[6])
+                 : launch(own_tokens_kernel<false, 2, 1>, own_smem<2, 1>(), 64, done[7]);
+  }
+  if (rc != NE_OK) return rc;
   const long long vectors = (long long)rows.max_q_len * nh;
   return launch_kernel(join_kernel, dim3(rows.num_seqs, (unsigned)((vectors + JOIN_WARPS - 1) / JOIN_WARPS)),
-                       dim3(32 * JOIN_WARPS), 0, stream, out, rows, groups, nh, nkv, parts, sms) == cudaSuccess
+                       dim3(32 * JOIN_WARPS), 0, stream, out, rows, groups, nh, nkv, parts) == cudaSuccess
              ? NE_OK
              : NE_ERR_CUDA;
 }
@@ -1158,9 +1251,9 @@ extern "C" NE_API size_t ne_prefix_attention_workspace_bytes(int max_rows, int n
       !ne::heads_ok(num_heads, num_kv_heads) || max_q_len < 1 || max_context < 0)
     return 0;
   const int sms = ne::device_sms();
-  const int tiles = (int)(((long long)max_q_len * (num_heads / num_kv_heads) + 15) / 16);
+  const int chunks = ne::own_chunks(max_q_len, num_heads / num_kv_heads);
   return ne::layout_of(max_rows, num_seqs, num_groups, num_heads,
-                       ne::own_splits(num_seqs, num_kv_heads, tiles, max_context, sms), sms).total;
+                       ne::own_splits(num_seqs, num_kv_heads, chunks, max_context, sms), sms).total;
 }
 
 extern "C" NE_API int ne_prefix_attention(const void* q, void* out, const void* k_cache, const void* v_cache,
