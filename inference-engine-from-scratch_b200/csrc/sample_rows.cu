@@ -8,9 +8,10 @@
 // and at least 1. The token is the first kept id, in ascending order, whose prefix mass exceeds
 // u times the kept mass.
 //
-// A row is a cluster of CTAs, each with a slice of the row in shared memory as ordered integer keys
-// (larger key = larger logit), so the logits are read from memory once. Cuts are found by a radix
-// select over the keys, 1024 bins a pass, counts and masses added over the cluster. A border is
+// A row is a cluster of CTAs, each with a slice of the row in shared memory, so the logits are read
+// from memory once. Cuts are found by a radix select over ordered integer keys (larger key = larger
+// logit), 1024 bins a pass, counts and masses added over the cluster; a vector of 16 bytes whose
+// largest logit is below the search is passed over. A border is
 // decided by sums over the whole vocabulary, so weights are computed in 64 bits (an error of 1e-7
 // in a weight, as fp32 gives, moves the border of a flat distribution past a token) and summed as
 // 2^-45 fixed point, whose sums do not depend on their order: the same inputs give the same tokens.
@@ -27,18 +28,20 @@ namespace cg = cooperative_groups;
 constexpr int RT = 512;               // threads per CTA
 constexpr int RW = RT / 32;
 constexpr int BINS = 1024;
+constexpr int MOST = 2048;            // tokens of a list
 constexpr int MAX_CLUSTER = 8;
 constexpr unsigned ALL = 0xFFFFFFFFu;
 constexpr double FIX = 35184372088832.0;  // 2^45
 constexpr int MAX_VOCAB = 1 << 18;        // 262,144 weights of at most 1 sum to at most 2^63
-constexpr size_t MAX_SLICE_BYTES = 200 << 10;
+constexpr size_t MAX_SLICE_BYTES = 132 << 10;  // MAX_VOCAB / MAX_CLUSTER tokens in fp32, and a padded vector
 
 // Ordered key of a logit, in the low bits: 16 for bf16, 32 for fp32. NaN and -inf: never drawn.
+// A vector is 16 bytes of a row; ``top`` is its largest logit (NaN aside).
 template <typename T>
 struct Keys;
 template <>
 struct Keys<__nv_bfloat16> {
-  using Raw = uint16_t;
+  static constexpr int PER = 8;
   static constexpr uint32_t NONE = 0x007Fu;  // the key of -inf; keys up to it hold no token
   static __device__ __forceinline__ uint32_t key(uint32_t b) {
     if ((b & 0x7FFFu) > 0x7F80u) return 0u;  // NaN
@@ -49,13 +52,26 @@ struct Keys<__nv_bfloat16> {
     const uint32_t b = (k & 0x8000u) ? (k & 0x7FFFu) : (~k & 0xFFFFu);
     return __uint_as_float(b << 16);
   }
-  static __device__ __forceinline__ uint32_t floor_key(float x) {  // a key no larger than any logit >= x has
-    return key(__float_as_uint(x) >> 16);                          // (truncated towards 0: rounded down below)
+  static __device__ __forceinline__ uint32_t key_of(float x) { return key(__float_as_uint(x) >> 16); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
   }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ uint32_t at(const uint4& v, int j) {  // (j a constant)
+    const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+    return key(j & 1 ? w >> 16 : w & 0xFFFFu);
+  }
+  static constexpr uint16_t PAD = 0xFF80u;  // -inf
+  using Raw = uint16_t;
 };
 template <>
 struct Keys<float> {
-  using Raw = uint32_t;
+  static constexpr int PER = 4;
   static constexpr uint32_t NONE = 0x007FFFFFu;
   static __device__ __forceinline__ uint32_t key(uint32_t b) {
     if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0u;
@@ -65,17 +81,38 @@ struct Keys<float> {
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
   }
-  static __device__ __forceinline__ uint32_t floor_key(float x) { return key(__float_as_uint(x)); }
+  static __device__ __forceinline__ uint32_t key_of(float x) { return key(__float_as_uint(x)); }
+  static __device__ __forceinline__ float top(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ uint32_t at(const uint4& v, int j) {
+    return key(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w);
+  }
+  static constexpr uint32_t PAD = 0xFF800000u;
+  using Raw = uint32_t;
 };
 
+// Fixed-point masses of a bin in three 15-bit pieces: a CTA's 2^15 tokens of at most 2^45 add up in 32
+// bits each, by the 32-bit shared-memory atomics (a 64-bit one took a pass from 15 to 90 us a row).
+struct Bins {
+  uint32_t count[BINS], piece[3][BINS];
+};
+// The tokens at or above a lower bound of all cuts, where they are few: gathered into the first CTA.
+struct List {
+  unsigned long long entry[MOST], mass[MOST];
+};
 struct Shared {
-  unsigned long long mass[2][BINS];
-  uint32_t count[2][BINS];
+  union {
+    Bins bins[2];
+    List list;
+  };
   unsigned long long red64[RW];
   uint32_t red32[RW];
+  double pow2[32];
   // published to the cluster
-  unsigned long long pub_best, pub_sum;
-  uint32_t pub_low[2], pub_ties;
+  unsigned long long pub_sum;
+  uint32_t pub_best, pub_low[2], pub_ties, pub_listed;
+  int pub_id;
   // the bin a select pass chose
   int sel_bin;
   uint32_t sel_count;
@@ -92,17 +129,47 @@ struct Cut {
 
 template <typename T>
 struct Row {
-  const typename Keys<T>::Raw* keys;  // this CTA's slice
-  int n;                              // its tokens
-  uint32_t top;                       // the row's largest key
-  double m, temp;                     // its value; the temperature
+  const uint4* vecs;   // this CTA's slice: vector v holds tokens PER v .. of it, padded with -inf
+  int count;           // its vectors
+  uint32_t top;        // the row's largest key
+  double m, scale;     // its value; log2(e) / temperature
+  const double* pow2;  // 2^(i / 32)
 
+  // exp((x - m) / T) = 2^t, t = n / 32 + r, |r| <= 1/64: the table's 2^(n / 32) times the series of 2^r
+  // to the fifth power (an error of 2e-15, and the rounding of t: below 1e-13 in all)
   __device__ __forceinline__ double weight(uint32_t k) const {
-    if (k == top) return 1.0;
-    if (k <= Keys<T>::NONE) return 0.0;
-    return exp(((double)Keys<T>::value(k) - m) / temp);
+    const double t0 = ((double)Keys<T>::value(k) - m) * scale;
+    const double t = t0 > -60.0 ? t0 : -60.0;  // (2^-60 is below half a step of the fixed point)
+    constexpr double MAGIC = 6755399441055744.0 / 32.0;  // 1.5 x 2^52 / 32: t rounded to 1 / 32
+    const double u = t + MAGIC;
+    const int n = __double2loint(u);
+    const double r = t - (u - MAGIC);
+    double y = 0.0013333558146428443;
+    y = fma(y, r, 0.009618129107628477);
+    y = fma(y, r, 0.05550410866482158);
+    y = fma(y, r, 0.2402265069591007);
+    y = fma(y, r, 0.6931471805599453);
+    const double p = pow2[n & 31];
+    y = fma(y * r, p, p);
+    y = __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y));
+    return k == top ? 1.0 : k <= Keys<T>::NONE ? 0.0 : y;  // (an infinite top: 1 for it, 0 for the rest)
   }
   __device__ __forceinline__ unsigned long long fixed(uint32_t k) const { return __double2ull_rn(weight(k) * FIX); }
+
+  // f(token of the slice, key) for every token with a key of at least ``lo`` (above NONE)
+  template <typename F>
+  __device__ __forceinline__ void above(uint32_t lo, F&& f) const {
+    const float least = Keys<T>::value(lo);
+    for (int v = threadIdx.x; v < count; v += RT) {
+      const uint4 x = vecs[v];
+      if (!(Keys<T>::top(x) >= least)) continue;
+#pragma unroll
+      for (int j = 0; j < Keys<T>::PER; ++j) {
+        const uint32_t k = Keys<T>::at(x, j);
+        if (k >= lo) f(v * Keys<T>::PER + j, k);
+      }
+    }
+  }
 };
 
 __device__ __forceinline__ unsigned long long warp_add(unsigned long long v) {
@@ -141,29 +208,40 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
   for (;;) {
     const uint32_t range = hi - lo;
     const int shift = max(0, 32 - __clz(range) - 10);
+    Bins& bins = sh.bins[buf];
     for (int i = threadIdx.x; i < BINS; i += RT) {
-      sh.count[buf][i] = 0u;
-      if (MASS) sh.mass[buf][i] = 0ull;
+      bins.count[i] = 0u;
+      if (MASS) bins.piece[0][i] = bins.piece[1][i] = bins.piece[2][i] = 0u;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < row.n; i += RT) {
-      const uint32_t k = row.keys[i];
-      if (k < lo || k > hi || k <= Keys<T>::NONE) continue;
+    row.above(max(lo, Keys<T>::NONE + 1u), [&](int, uint32_t k) {
+      if (k > hi) return;
       const uint32_t b = (k - lo) >> shift;
-      atomicAdd(&sh.count[buf][b], 1u);
-      if (MASS) atomicAdd(&sh.mass[buf][b], row.fixed(k));
-    }
+      atomicAdd(&bins.count[b], 1u);
+      if (MASS) {
+        const unsigned long long f = row.fixed(k);
+        atomicAdd(&bins.piece[0][b], (uint32_t)f & 0x7FFFu);
+        atomicAdd(&bins.piece[1][b], (uint32_t)(f >> 15) & 0x7FFFu);
+        atomicAdd(&bins.piece[2][b], (uint32_t)(f >> 30));
+      }
+    });
     cl.sync();
     // every CTA adds the cluster's bins: thread t owns bins 2 t and 2 t + 1
     uint32_t c[2] = {0u, 0u};
     unsigned long long w[2] = {0ull, 0ull};
+#pragma unroll 4
     for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-      const uint32_t* rc = cl.map_shared_rank(&sh.count[buf][0], r);
-      const unsigned long long* rm = cl.map_shared_rank(&sh.mass[buf][0], r);
+      const Bins* remote = cl.map_shared_rank(&bins, r);
+      const uint2 rc = reinterpret_cast<const uint2*>(remote->count)[threadIdx.x];
+      c[0] += rc.x;
+      c[1] += rc.y;
+      if (MASS) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        c[j] += rc[2 * threadIdx.x + j];
-        if (MASS) w[j] += rm[2 * threadIdx.x + j];
+        for (int q = 0; q < 3; ++q) {
+          const uint2 rp = reinterpret_cast<const uint2*>(remote->piece[q])[threadIdx.x];
+          w[0] += (unsigned long long)rp.x << (15 * q);
+          w[1] += (unsigned long long)rp.y << (15 * q);
+        }
       }
     }
     const unsigned long long v[2] = {MASS ? w[0] : c[0], MASS ? w[1] : c[1]};
@@ -226,8 +304,117 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
   return cut;
 }
 
+// Ascending (UP) or descending bitonic sort of the first ``size`` (a power of two) entries, by the CTA.
+template <bool UP>
+__device__ void sort_entries(unsigned long long* e, int size) {
+  for (int width = 2; width <= size; width *= 2) {
+    for (int stride = width / 2; stride > 0; stride /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += RT) {
+        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+        const unsigned long long a = e[lo], b = e[hi];
+        if ((a > b) == (((lo & width) == 0) == UP)) {
+          e[lo] = b;
+          e[hi] = a;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Inclusive prefix sums of f(0), f(1), .. f(size - 1) (size a power of two up to MOST): each thread gets
+// its entries' in ``out``, thread t entries t * per .. of them; block-wide, returns per.
+template <typename F>
+__device__ int scan_entries(Shared& sh, int size, F&& f, unsigned long long (&out)[MOST / RT]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = max(1, size / RT);
+  unsigned long long run = 0;
+#pragma unroll
+  for (int i = 0; i < MOST / RT; ++i) {
+    const int at = threadIdx.x * per + i;
+    if (i < per && at < size) run += f(at);
+    out[i] = run;
+  }
+  unsigned long long incl = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long t = __shfl_up_sync(ALL, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();
+  if (lane == 31) sh.red64[warp] = incl;
+  __syncthreads();
+  unsigned long long before = incl - run;
+  for (int w = 0; w < warp; ++w) before += sh.red64[w];
+#pragma unroll
+  for (int i = 0; i < MOST / RT; ++i) out[i] += before;
+  return per;
+}
+
+// Everything behind the list, by the first CTA alone: the cuts are places in the sorted list, and the
+// draw is a second sort, of the kept tokens by id.
 template <typename T>
-__global__ void __launch_bounds__(RT)
+__device__ void draw_from_list(Shared& sh, const Row<T>& row, int n, int k, float tp, double floor_w, float u,
+                               int32_t* token, float* prob) {
+  List& list = sh.list;
+  int size = 32;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += RT) list.entry[i] = 0ull;
+  __syncthreads();
+  sort_entries<false>(list.entry, size);  // largest key first, lowest id first among equals
+  const int n_k = k > 0 ? min(k, n) : n;
+  for (int i = threadIdx.x; i < size; i += RT)
+    list.mass[i] = i < n_k ? row.fixed((uint32_t)(list.entry[i] >> 32)) : 0ull;
+  __syncthreads();
+  unsigned long long sum[MOST / RT];
+  int per = scan_entries(sh, size, [&](int i) { return list.mass[i]; }, sum);
+  // the number of kept tokens: those that start below the limit and weigh enough (each a prefix)
+  unsigned long long limit = ~0ull;
+  if (tp < 1.f) {
+    unsigned long long z = 0;
+    for (int w = 0; w < RW; ++w) z += sh.red64[w];
+    const double edge = ceil((double)fmaxf(tp, 0.f) * (double)z);
+    limit = edge < 1.0 ? 1ull : (unsigned long long)edge;
+  }
+  int kept = 0;
+#pragma unroll
+  for (int i = 0; i < MOST / RT; ++i) {
+    const int at = threadIdx.x * per + i;
+    if (i < per && at < n_k)
+      kept += sum[i] - list.mass[at] < limit && row.weight((uint32_t)(list.entry[at] >> 32)) >= floor_w;
+  }
+  kept = __reduce_add_sync(ALL, kept);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.red32[threadIdx.x >> 5] = kept;
+  __syncthreads();
+  kept = 0;
+  for (int w = 0; w < RW; ++w) kept += sh.red32[w];
+  kept = max(kept, 1);
+  // the kept tokens by id: id in the upper bits, the place in the sorted list below
+  size = 32;
+  while (size < kept) size *= 2;
+  for (int i = threadIdx.x; i < size; i += RT)
+    list.entry[i] = i < kept ? (unsigned long long)(0xFFFFFFFFu - (uint32_t)list.entry[i]) << 32 | i : ~0ull;
+  __syncthreads();
+  sort_entries<true>(list.entry, size);
+  per = scan_entries(sh, size, [&](int i) { return i < kept ? list.mass[(uint32_t)list.entry[i]] : 0ull; }, sum);
+  unsigned long long total = 0;
+  for (int w = 0; w < RW; ++w) total += sh.red64[w];
+  const double want = u > 0.f ? floor((double)u * (double)total) : 0.0;
+  const unsigned long long target = want >= (double)total ? total - 1ull : (unsigned long long)want;
+#pragma unroll
+  for (int i = 0; i < MOST / RT; ++i) {
+    const int at = threadIdx.x * per + i;
+    if (i >= per || at >= kept) continue;
+    const unsigned long long w = list.mass[(uint32_t)list.entry[at]];
+    if (sum[i] > target && sum[i] - w <= target) {
+      *token = (int32_t)(list.entry[at] >> 32);
+      if (prob) *prob = (float)((double)w / (double)total);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(RT, 2)
     sample_rows_kernel(const T* __restrict__ logits, long long row_stride, int vocab, int slice,
                        const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
                        const float* __restrict__ top_p, const float* __restrict__ min_p,
@@ -243,115 +430,133 @@ __global__ void __launch_bounds__(RT)
   const int r = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = min(vocab, rank * slice), n = min(vocab, first + slice) - first;
+  if (tid < 32) sh.pow2[tid] = exp2((double)tid * (1.0 / 32.0));
 
-  // ---- the slice into shared memory, as keys; 16-byte loads from the first aligned logit on
-  constexpr int PER = 16 / sizeof(Raw);
+  // ---- the slice into shared memory; 16-byte loads from the first aligned logit on. Vector 0 of the
+  // slice starts at that boundary's token or before: ``skew`` places of it are padding
+  constexpr int PER = K::PER;
   const Raw* src = reinterpret_cast<const Raw*>(logits) + (long long)r * row_stride + first;
-  const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15u) / sizeof(Raw));  // tokens past a boundary
-  Raw* keys = reinterpret_cast<Raw*>(slice_smem) + skew;
-  const int head = min(n, (PER - skew) & (PER - 1));
-  const int vecs = (n - head) / PER;
-  uint32_t top = 0u;
-  int top_at = 0;
-  auto take = [&](int i, uint32_t raw) {
-    const uint32_t k = K::key(raw);
-    if (k > top) {
-      top = k;
-      top_at = i;
-    }
-    return (Raw)k;
-  };
-  if (tid < head) keys[tid] = take(tid, src[tid]);
-  const uint4* vsrc = reinterpret_cast<const uint4*>(src + head);
+  const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15u) / sizeof(Raw));
+  uint4* vecs = reinterpret_cast<uint4*>(slice_smem);
+  const int count = n > 0 ? (skew + n + PER - 1) / PER : 0;
+  const uint4* vsrc = reinterpret_cast<const uint4*>(src - skew);
+  float top = -INFINITY;
 #pragma unroll 4
-  for (int v = tid; v < vecs; v += RT) {
-    const uint4 x = vsrc[v];
-    union {
-      uint4 v;
-      Raw e[PER];
-    } in, out;
-    in.v = x;
+  for (int v = tid; v < count; v += RT) {
+    uint4 x;
+    if ((v > 0 || skew == 0) && (v + 1) * PER <= skew + n) {
+      x = vsrc[v];
+    } else {  // the first or last vector, in part
+      union {
+        uint4 v;
+        Raw e[PER];
+      } part;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) out.e[j] = take(head + v * PER + j, in.e[j]);
-    *reinterpret_cast<uint4*>(keys + head + v * PER) = out.v;
+      for (int j = 0; j < PER; ++j) {
+        const int i = v * PER + j - skew;
+        part.e[j] = i >= 0 && i < n ? src[i] : K::PAD;
+      }
+      x = part.v;
+    }
+    vecs[v] = x;
+    top = fmaxf(top, K::top(x));
   }
-  for (int i = head + vecs * PER + tid; i < n; i += RT) keys[i] = take(i, src[i]);
 
-  // ---- the row's largest key (lowest id among equals), and lower bounds that hold 1 token each
-  unsigned long long best = ((unsigned long long)top << 32) | (0xFFFFFFFFu - (uint32_t)(first + top_at));
-  const uint32_t thread_low = __reduce_min_sync(ALL, top);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long t = __shfl_xor_sync(ALL, best, o);
-    best = t > best ? t : best;
-  }
+  // ---- the row's largest logit, and lower bounds that hold a token each
+  const uint32_t thread_top = K::key_of(top);
+  const uint32_t warp_top = __reduce_max_sync(ALL, thread_top), thread_low = __reduce_min_sync(ALL, thread_top);
   if (lane == 0) {
-    sh.red64[warp] = best;
-    sh.red32[warp] = thread_low;
+    sh.red64[warp] = (unsigned long long)warp_top << 32 | thread_low;
   }
   __syncthreads();
   if (tid == 0) {
-    unsigned long long b = 0;
-    uint32_t wl = 0xFFFFFFFFu, tl = 0xFFFFFFFFu;
+    uint32_t best = 0u, wl = 0xFFFFFFFFu, tl = 0xFFFFFFFFu;
     for (int w = 0; w < RW; ++w) {
-      b = sh.red64[w] > b ? sh.red64[w] : b;
-      wl = min(wl, (uint32_t)(sh.red64[w] >> 32));
-      tl = min(tl, sh.red32[w]);
+      const uint32_t wt = (uint32_t)(sh.red64[w] >> 32);
+      best = max(best, wt);
+      wl = min(wl, wt);
+      tl = min(tl, (uint32_t)sh.red64[w]);
     }
-    sh.pub_best = b;
+    sh.pub_best = best;
     sh.pub_low[0] = wl;
     sh.pub_low[1] = tl;
+    sh.pub_id = 0x7FFFFFFF;
+    sh.pub_listed = 0u;
   }
   cl.sync();
-  uint32_t low[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-  best = 0;
+  uint32_t low[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, row_top = 0u;
   for (int q = 0; q < ctas; ++q) {
-    const unsigned long long b = *cl.map_shared_rank(&sh.pub_best, q);
-    best = b > best ? b : best;
+    row_top = max(row_top, *cl.map_shared_rank(&sh.pub_best, q));
     const uint32_t* l = cl.map_shared_rank(&sh.pub_low[0], q);
     low[0] = min(low[0], l[0]);
     low[1] = min(low[1], l[1]);
   }
-  const uint32_t row_top = (uint32_t)(best >> 32);
+  Row<T> row;
+  row.vecs = vecs;
+  row.count = count;
+  row.top = row_top;
+  row.m = (double)K::value(row_top);
+  row.pow2 = sh.pow2;
   const float T_row = temperature ? temperature[r] : 1.f;
+  row.scale = 1.4426950408889634 / (double)T_row;
   const bool empty = row_top <= K::NONE;
-  if (empty || !(T_row > 0.f)) {  // nothing to draw, or greedy: the largest logit
+  if (empty || !(T_row > 0.f)) {  // nothing to draw, or greedy: the lowest id of the largest logit
+    if (!empty) {
+      row.above(row_top, [&](int i, uint32_t) { atomicMin(cl.map_shared_rank(&sh.pub_id, 0), first + i - skew); });
+    }
+    cl.sync();
     if (rank == 0 && tid == 0) {
-      tokens[r] = empty ? -1 : (int32_t)(0xFFFFFFFFu - (uint32_t)best);
+      tokens[r] = empty ? -1 : sh.pub_id;
       if (probs) probs[r] = empty ? 0.f : 1.f;
       if (empty) report(status, NE_DEV_BAD_TOKEN);
     }
-    cl.sync();  // (no CTA leaves while another may read its shared memory)
     return;
   }
-  Row<T> row;
-  row.keys = keys;
-  row.n = n;
-  row.top = row_top;
-  row.m = (double)K::value(row_top);
-  row.temp = (double)T_row;
 
   // ---- the cuts
   const int k = top_k ? top_k[r] : 0;
   const float tp = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
+  const double floor_w = mp > 0.f ? (double)mp : 0.0;
+  const bool some = k > 0 && k < vocab;
+  // A lower bound of all cuts. ctas * RW warps each hold a token of at least the lowest warp maximum:
+  // with so many of them or fewer the k-th largest is no lower. Without top-p, whose mass counts the
+  // tokens that min-p cuts, min-p is a bound too (a key lower for the rounding of the logarithm).
+  uint32_t bound = some && k <= ctas * RW ? low[0] : 0u;
+  if (mp > 0.f && !(tp < 1.f)) {
+    const double x0 = row.m + (double)T_row * log(fmin(floor_w, 1.0));
+    const uint32_t f = x0 > -3.0e38 ? K::key_of(__double2float_rd(x0)) : 0u;
+    bound = max(bound, min(f > 0u ? f - 1u : 0u, row_top));
+  }
+  if (bound > K::NONE) {
+    uint32_t have = 0;
+    row.above(bound, [&](int, uint32_t) { ++have; });
+    const unsigned long long n_list = cluster_sum(cl, sh, have);
+    if (n_list <= MOST) {
+      row.above(bound, [&](int i, uint32_t key) {
+        const uint32_t at = atomicAdd(cl.map_shared_rank(&sh.pub_listed, 0), 1u);
+        cl.map_shared_rank(&sh.list, 0)->entry[at] =
+            (unsigned long long)key << 32 | (0xFFFFFFFFu - (uint32_t)(first + i - skew));
+      });
+      cl.sync();
+      if (rank == 0)
+        draw_from_list(sh, row, (int)n_list, some ? k : 0, tp, floor_w, uniform[r], tokens + r, probs ? probs + r : nullptr);
+      return;
+    }
+  }
   Cut cut{K::NONE + 1u, 0xFFFFFFFFu, 0u};  // every token (all ties of the lowest key)
-  bool partial = false;                    // the cut divides its ties
   if (mp > 1.f) {
     cut = select_cut<T, false>(cl, sh, row, row_top, row_top, 1ull);
   } else {
-    if (k > 0 && k < vocab) {
-      // ctas * RW warps (ctas * RT threads) each hold a token of at least the lowest warp (thread)
-      // maximum: with k of them or fewer the k-th largest is no lower
+    if (some) {  // (the threads' maxima bound the k-th largest as the warps' do)
       uint32_t lo = k <= ctas * RW ? low[0] : k <= ctas * RT ? low[1] : 0u;
       lo = max(lo, K::NONE + 1u);
       cut = select_cut<T, false>(cl, sh, row, lo, row_top, (unsigned long long)k);
     }
     if (tp < 1.f) {
       unsigned long long z = 0;
-      for (int i = tid; i < n; i += RT) {
-        const uint32_t key = keys[i];
-        if (key > cut.key || (key == cut.key && !cut.ties)) z += row.fixed(key);
-      }
+      row.above(cut.key, [&](int, uint32_t key) {
+        if (key > cut.key || !cut.ties) z += row.fixed(key);
+      });
       z = cluster_sum(cl, sh, z);
       if (cut.ties) z += (unsigned long long)cut.keep * row.fixed(cut.key);
       const double edge = ceil((double)fmaxf(tp, 0.f) * (double)z);
@@ -360,25 +565,28 @@ __global__ void __launch_bounds__(RT)
       // at or above w0 (taken a little lower for the rounding of the logarithm)
       const double w0 = (1.0 - (double)fmaxf(tp, 0.f)) * ((double)z / FIX) / vocab * 0.999;
       uint32_t lo = cut.key;
-      const double x0 = row.m + row.temp * log(w0);
+      const double x0 = row.m + (double)T_row * log(w0);
       if (x0 > -3.0e38) {
-        const float xf = __double2float_rd(x0);
-        uint32_t f = K::floor_key(xf);
-        f = f > 0u ? f - 1u : 0u;
-        lo = max(lo, min(f, row_top));
+        const uint32_t f = K::key_of(__double2float_rd(x0));
+        lo = max(lo, min(f > 0u ? f - 1u : 0u, row_top));
       }
       cut = select_cut<T, true>(cl, sh, row, lo, row_top, limit);
     }
   }
-  partial = cut.ties != 0u && cut.keep < cut.ties;
-  const double floor_w = mp > 0.f && mp <= 1.f ? (double)mp : 0.0;
+  const bool partial = cut.ties != 0u && cut.keep < cut.ties;  // the cut divides its ties
 
-  // ---- the draw: warp w of CTA c walks the w-th part of slice c in ascending id order
-  const int len = ((n + RT - 1) / RT) * 32, begin = min(n, warp * len), end = min(n, begin + len);
+  // ---- the draw: warp w of CTA c walks the w-th part of slice c, a vector a lane, in ascending id order
+  const int len = (count + RW - 1) / RW, begin = min(count, warp * len), end = min(count, begin + len);
+  const float least = K::value(cut.key);
   uint32_t tie_base = 0;
   if (partial) {  // ties before this warp's part
     uint32_t ties = 0;
-    for (int i = begin + lane; i < end; i += 32) ties += keys[i] == cut.key;
+    for (int v = begin + lane; v < end; v += 32) {
+      const uint4 x = vecs[v];
+      if (!(K::top(x) >= least)) continue;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) ties += K::at(x, j) == cut.key;
+    }
     ties = __reduce_add_sync(ALL, ties);
     __syncthreads();
     if (lane == 0) sh.red32[warp] = ties;
@@ -392,21 +600,49 @@ __global__ void __launch_bounds__(RT)
     cl.sync();
     for (int q = 0; q < rank; ++q) tie_base += *cl.map_shared_rank(&sh.pub_ties, q);
   }
-  // token i's mass if it is kept (``rank_at``: ties before it); warp-collective
-  auto kept_mass = [&](int i, uint32_t& rank_at) -> unsigned long long {
-    const bool in = i < end;
-    const uint32_t key = in ? (uint32_t)keys[i] : 0u;
-    const uint32_t tie = __ballot_sync(ALL, in && key == cut.key);
-    bool keep = in && key > cut.key;
-    if (in && key == cut.key) keep = !partial || rank_at + __popc(tie & ((1u << lane) - 1u)) < cut.keep;
-    rank_at += __popc(tie);
-    if (!keep) return 0ull;
-    const double w = row.weight(key);
-    return w >= floor_w ? __double2ull_rn(w * FIX) : 0ull;
+  // the kept mass of a lane's vector (``ranked``: ties before it); each(j, mass) in id order
+  auto kept = [&](const uint4& x, uint32_t ranked, auto&& each) {
+    if (!(K::top(x) >= least)) return;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t key = K::at(x, j);
+      if (key < cut.key) continue;
+      if (key == cut.key && partial && ranked++ >= cut.keep) continue;
+      const double w = row.weight(key);
+      if (w >= fmin(floor_w, 1.0)) each(j, __double2ull_rn(w * FIX));
+    }
   };
+  // ties in the lanes before this one's, and in all of them (only where the cut divides its ties)
+  auto rank_of = [&](const uint4& x, uint32_t& before) -> uint32_t {
+    if (!partial) return 0u;
+    uint32_t mine = 0;
+    if (K::top(x) >= least) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) mine += K::at(x, j) == cut.key;
+    }
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t t = __shfl_up_sync(ALL, incl, o);
+      if (lane >= o) incl += t;
+    }
+    const uint32_t at = before + incl - mine;
+    before += __shfl_sync(ALL, incl, 31);
+    return at;
+  };
+  union {
+    Raw e[PER];
+    uint4 v;
+  } none;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) none.e[j] = K::PAD;
   unsigned long long sum = 0;
-  uint32_t at = tie_base;
-  for (int b = begin; b < end; b += 32) sum += kept_mass(b + lane, at);
+  uint32_t before_ties = tie_base;
+  for (int b = begin; b < end; b += 32) {
+    const uint4 x = b + lane < end ? vecs[b + lane] : none.v;
+    const uint32_t ranked = rank_of(x, before_ties);
+    kept(x, ranked, [&](int, unsigned long long w) { sum += w; });
+  }
   sum = warp_add(sum);
   __syncthreads();
   if (lane == 0) sh.red64[warp] = sum;
@@ -426,10 +662,13 @@ __global__ void __launch_bounds__(RT)
   const double want = u > 0.f ? floor((double)u * (double)total) : 0.0;
   const unsigned long long target = want >= (double)total ? total - 1ull : (unsigned long long)want;
   if (before <= target && before + sum > target) {  // one warp of the cluster
-    at = tie_base;
+    before_ties = tie_base;
     unsigned long long run = before;
     for (int b = begin; b < end; b += 32) {
-      const unsigned long long w = kept_mass(b + lane, at);
+      const uint4 x = b + lane < end ? vecs[b + lane] : none.v;
+      const uint32_t ranked = rank_of(x, before_ties);
+      unsigned long long w = 0;
+      kept(x, ranked, [&](int, unsigned long long f) { w += f; });
       unsigned long long incl = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -439,15 +678,22 @@ __global__ void __launch_bounds__(RT)
       const uint32_t hit = __ballot_sync(ALL, run + incl > target);
       if (hit) {
         if (lane == __ffs(hit) - 1) {
-          tokens[r] = first + b + lane;
-          if (probs) probs[r] = (float)((double)w / (double)total);
+          unsigned long long at = run + incl - w;
+          bool done = false;
+          kept(x, ranked, [&](int j, unsigned long long f) {
+            at += f;
+            if (done || at <= target) return;
+            done = true;
+            tokens[r] = first - skew + (b + lane) * PER + j;
+            if (probs) probs[r] = (float)((double)f / (double)total);
+          });
         }
         break;
       }
       run += __shfl_sync(ALL, incl, 31);
     }
   }
-  cl.sync();
+  cl.sync();  // (no CTA leaves while another may read its shared memory)
 }
 
 template <typename T>
@@ -458,7 +704,7 @@ int launch_sample_rows(const void* logits, int rows, int vocab, long long row_st
   // about 8,192 tokens a CTA: below that the cluster's barriers cost more than the shorter slices save
   while (ctas < MAX_CLUSTER && vocab > 8192 * ctas) ctas *= 2;
   const int slice = (vocab + ctas - 1) / ctas;
-  const size_t smem = ((size_t)slice + 16) * sizeof(T);
+  const size_t smem = ((size_t)slice * sizeof(T) + 47) / 16 * 16;  // (a padded vector at either end)
   if (smem > MAX_SLICE_BYTES) return NE_ERR_UNSUPPORTED;
   static bool done[64] = {};
   int dev = 0;
