@@ -12,9 +12,9 @@
 // from memory once. Cuts are found by a radix select over ordered integer keys (larger key = larger
 // logit), 1024 bins a pass, counts and masses added over the cluster; a vector of 16 bytes whose
 // largest logit is below the search is passed over. A border is
-// decided by sums over the whole vocabulary, so weights are computed in 64 bits (an error of 1e-7
-// in a weight, as fp32 gives, moves the border of a flat distribution past a token) and summed as
-// 2^-45 fixed point, whose sums do not depend on their order: the same inputs give the same tokens.
+// decided by sums over the whole vocabulary, so weights are good to about 2e-9 (an error of 1e-7, as
+// plain fp32 gives, moves the border of a flat distribution past a token) and summed in steps of 2^-45,
+// whose sums do not depend on their order: the same inputs give the same tokens.
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"
@@ -31,7 +31,8 @@ constexpr int BINS = 1024;
 constexpr int MOST = 2048;            // tokens of a list
 constexpr int MAX_CLUSTER = 8;
 constexpr unsigned ALL = 0xFFFFFFFFu;
-constexpr double FIX = 35184372088832.0;  // 2^45
+constexpr double FIX = 35184372088832.0;          // 2^45
+constexpr unsigned long long ONE = 1ull << 45;    // a weight of 1
 constexpr int MAX_VOCAB = 1 << 18;        // 262,144 weights of at most 1 sum to at most 2^63
 constexpr size_t MAX_SLICE_BYTES = 132 << 10;  // MAX_VOCAB / MAX_CLUSTER tokens in fp32, and a padded vector
 
@@ -66,6 +67,10 @@ struct Keys<__nv_bfloat16> {
     const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
     return key(j & 1 ? w >> 16 : w & 0xFFFFu);
   }
+  static __device__ __forceinline__ float logit(const uint4& v, int j) {
+    const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+    return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+  }
   static constexpr uint16_t PAD = 0xFF80u;  // -inf
   using Raw = uint16_t;
 };
@@ -88,6 +93,9 @@ struct Keys<float> {
   static __device__ __forceinline__ uint32_t at(const uint4& v, int j) {
     return key(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w);
   }
+  static __device__ __forceinline__ float logit(const uint4& v, int j) {
+    return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w);
+  }
   static constexpr uint32_t PAD = 0xFF800000u;
   using Raw = uint32_t;
 };
@@ -108,10 +116,12 @@ struct Shared {
   };
   unsigned long long red64[RW];
   uint32_t red32[RW];
-  double pow2[32];
+  uint2 pow2[64];  // 2^(31 + i / 64) in 32 bits (2^32 - 1 at most), and an eighth of it as a float
   // published to the cluster
   unsigned long long pub_sum;
-  uint32_t pub_best, pub_low[2], pub_ties, pub_listed;
+  uint32_t pub_best, pub_low, pub_ties, pub_listed, bound;
+  uint32_t pub_tops[4 * RW];               // the largest key of each quarter warp
+  alignas(16) uint32_t tops[4 * RW * MAX_CLUSTER];  // (the cluster's)
   int pub_id;
   // the bin a select pass chose
   int sel_bin;
@@ -132,29 +142,50 @@ struct Row {
   const uint4* vecs;   // this CTA's slice: vector v holds tokens PER v .. of it, padded with -inf
   int count;           // its vectors
   uint32_t top;        // the row's largest key
-  double m, scale;     // its value; log2(e) / temperature
-  const double* pow2;  // 2^(i / 32)
+  bool inf;            // it is infinite
+  float least;         // a logit whose weight is 2^-60
+  float c1, c2;        // log2(e) / temperature = c1 + c2
+  float mp, me, ml;    // the largest logit times c1 (its product, and the rounding error of that) and c2
+  const uint2* pow2;
 
-  // exp((x - m) / T) = 2^t, t = n / 32 + r, |r| <= 1/64: the table's 2^(n / 32) times the series of 2^r
-  // to the fifth power (an error of 2e-15, and the rounding of t: below 1e-13 in all)
-  __device__ __forceinline__ double weight(uint32_t k) const {
-    const double t0 = ((double)Keys<T>::value(k) - m) * scale;
-    const double t = t0 > -60.0 ? t0 : -60.0;  // (2^-60 is below half a step of the fixed point)
-    constexpr double MAGIC = 6755399441055744.0 / 32.0;  // 1.5 x 2^52 / 32: t rounded to 1 / 32
-    const double u = t + MAGIC;
-    const int n = __double2loint(u);
-    const double r = t - (u - MAGIC);
-    double y = 0.0013333558146428443;
-    y = fma(y, r, 0.009618129107628477);
-    y = fma(y, r, 0.05550410866482158);
-    y = fma(y, r, 0.2402265069591007);
-    y = fma(y, r, 0.6931471805599453);
-    const double p = pow2[n & 31];
-    y = fma(y * r, p, p);
-    y = __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y));
-    return k == top ? 1.0 : k <= Keys<T>::NONE ? 0.0 : y;  // (an infinite top: 1 for it, 0 for the rest)
+  // exp((x - m) / T) in steps of 2^-45: 2^t, t = (x - m) log2(e) / T = n / 64 + r, |r| <= 1/128, as the
+  // table's 2^(n / 64) times the series of 2^r to the fourth power. On the FMA and integer pipes: the
+  // products x c and m c are taken with their rounding errors, and their difference with its own, so
+  // that t is off by less than 2^-30; the weight by about 2e-9 of itself, each logit's differently.
+  // (The same in fp64 took a pass over a row from 6 to 25 us.) A logit below ``least``, -inf or NaN
+  // weighs 2^-60, which is 0.
+  __device__ __forceinline__ unsigned long long power(float logit) const {
+    const float x = fmaxf(logit, least);
+    // (the rounded operations by name: none may be contracted with another)
+    const float p = __fmul_rn(x, c1), e = fmaf(x, c1, -p);    // x c1 = p + e
+    const float s = __fsub_rn(p, mp), z = __fsub_rn(s, p);    // p - mp = s + err
+    const float err = __fsub_rn(__fsub_rn(p, __fsub_rn(s, z)), __fadd_rn(mp, z));
+    const float low = err + (__fsub_rn(e, me) + fmaf(x, c2, -ml));
+    constexpr float MAGIC = 196608.f;                         // 1.5 x 2^17: s rounded to 1 / 64
+    const float u = __fadd_rn(s, MAGIC);
+    const int n = __float_as_int(u) - 0x48400000;
+    const float r = __fsub_rn(s, __fsub_rn(u, MAGIC)) + low;
+    float y = fmaf(r, 0.009618129f, 0.05550411f);
+    y = fmaf(y, r, 0.24022651f);
+    y = fmaf(y, r, 0.69314718f) * r;                          // 2^r - 1
+    const uint2 t = pow2[n & 63];                             // 2^(31 + n / 64), and an eighth as a float
+    // (|y| < 0.0055: the product is below 2^22, where 1.5 x 2^23 rounds it to an integer)
+    const int i = __float_as_int(fmaf(y, __uint_as_float(t.y), 12582912.f)) - 0x4B400000;
+    return ((unsigned long long)(t.x + (uint32_t)(i * 8)) << 14) >> (unsigned)-(n >> 6);
   }
-  __device__ __forceinline__ unsigned long long fixed(uint32_t k) const { return __double2ull_rn(weight(k) * FIX); }
+  // (an infinite largest logit: all for it, nothing for the rest)
+  __device__ __forceinline__ unsigned long long fixed(uint32_t k) const {
+    if (inf) return k == top ? ONE : 0ull;
+    return k <= Keys<T>::NONE ? 0ull : power(Keys<T>::value(k));
+  }
+  // the mass of all tokens of a vector
+  __device__ __forceinline__ unsigned long long vector_mass(const uint4& v) const {
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int j = 0; j < Keys<T>::PER; ++j)
+      sum += inf ? fixed(Keys<T>::at(v, j)) : power(Keys<T>::logit(v, j));
+    return sum;
+  }
 
   // f(token of the slice, key) for every token with a key of at least ``lo`` (above NONE)
   template <typename F>
@@ -307,6 +338,24 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
 // Ascending (UP) or descending bitonic sort of the first ``size`` (a power of two) entries, by the CTA.
 template <bool UP>
 __device__ void sort_entries(unsigned long long* e, int size) {
+  if (size <= 64) {  // a pair a lane
+    if (threadIdx.x < 32) {
+      const int i = threadIdx.x;
+      for (int width = 2; width <= size; width *= 2) {
+        for (int stride = width / 2; stride > 0; stride /= 2) {
+          const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+          const unsigned long long a = i < size / 2 ? e[lo] : 0ull, b = i < size / 2 ? e[hi] : 0ull;
+          if (i < size / 2 && (a > b) == (((lo & width) == 0) == UP)) {
+            e[lo] = b;
+            e[hi] = a;
+          }
+          __syncwarp();
+        }
+      }
+    }
+    __syncthreads();
+    return;
+  }
   for (int width = 2; width <= size; width *= 2) {
     for (int stride = width / 2; stride > 0; stride /= 2) {
       for (int i = threadIdx.x; i < size / 2; i += RT) {
@@ -353,7 +402,7 @@ __device__ int scan_entries(Shared& sh, int size, F&& f, unsigned long long (&ou
 // Everything behind the list, by the first CTA alone: the cuts are places in the sorted list, and the
 // draw is a second sort, of the kept tokens by id.
 template <typename T>
-__device__ void draw_from_list(Shared& sh, const Row<T>& row, int n, int k, float tp, double floor_w, float u,
+__device__ void draw_from_list(Shared& sh, const Row<T>& row, int n, int k, float tp, unsigned long long floor_w, float u,
                                int32_t* token, float* prob) {
   List& list = sh.list;
   int size = 32;
@@ -380,7 +429,7 @@ __device__ void draw_from_list(Shared& sh, const Row<T>& row, int n, int k, floa
   for (int i = 0; i < MOST / RT; ++i) {
     const int at = threadIdx.x * per + i;
     if (i < per && at < n_k)
-      kept += sum[i] - list.mass[at] < limit && row.weight((uint32_t)(list.entry[at] >> 32)) >= floor_w;
+      kept += sum[i] - list.mass[at] < limit && list.mass[at] >= floor_w;
   }
   kept = __reduce_add_sync(ALL, kept);
   __syncthreads();
@@ -430,7 +479,10 @@ __global__ void __launch_bounds__(RT, 2)
   const int r = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = min(vocab, rank * slice), n = min(vocab, first + slice) - first;
-  if (tid < 32) sh.pow2[tid] = exp2((double)tid * (1.0 / 32.0));
+  if (tid < 64) {
+    const double v = rint(exp2(31.0 + (double)tid * (1.0 / 64.0)));
+    sh.pow2[tid] = make_uint2((uint32_t)v, __float_as_uint((float)(v * 0.125)));
+  }
 
   // ---- the slice into shared memory; 16-byte loads from the first aligned logit on. Vector 0 of the
   // slice starts at that boundary's token or before: ``skew`` places of it are padding
@@ -462,43 +514,48 @@ __global__ void __launch_bounds__(RT, 2)
     top = fmaxf(top, K::top(x));
   }
 
-  // ---- the row's largest logit, and lower bounds that hold a token each
-  const uint32_t thread_top = K::key_of(top);
-  const uint32_t warp_top = __reduce_max_sync(ALL, thread_top), thread_low = __reduce_min_sync(ALL, thread_top);
-  if (lane == 0) {
-    sh.red64[warp] = (unsigned long long)warp_top << 32 | thread_low;
-  }
+  // ---- the row's largest logit, and the largest of each eight lanes' tokens
+  uint32_t top_key = K::key_of(top);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top_key = max(top_key, __shfl_xor_sync(ALL, top_key, o));
+  if ((lane & 7) == 0) sh.pub_tops[4 * warp + (lane >> 3)] = top_key;
+  const uint32_t warp_top = __reduce_max_sync(ALL, top_key), thread_low = __reduce_min_sync(ALL, K::key_of(top));
+  if (lane == 0) sh.red64[warp] = (unsigned long long)warp_top << 32 | thread_low;
   __syncthreads();
   if (tid == 0) {
-    uint32_t best = 0u, wl = 0xFFFFFFFFu, tl = 0xFFFFFFFFu;
+    uint32_t best = 0u, tl = 0xFFFFFFFFu;
     for (int w = 0; w < RW; ++w) {
-      const uint32_t wt = (uint32_t)(sh.red64[w] >> 32);
-      best = max(best, wt);
-      wl = min(wl, wt);
+      best = max(best, (uint32_t)(sh.red64[w] >> 32));
       tl = min(tl, (uint32_t)sh.red64[w]);
     }
     sh.pub_best = best;
-    sh.pub_low[0] = wl;
-    sh.pub_low[1] = tl;
+    sh.pub_low = tl;
     sh.pub_id = 0x7FFFFFFF;
     sh.pub_listed = 0u;
+    sh.bound = 0u;
   }
   cl.sync();
-  uint32_t low[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}, row_top = 0u;
+  uint32_t low = 0xFFFFFFFFu, row_top = 0u;
   for (int q = 0; q < ctas; ++q) {
     row_top = max(row_top, *cl.map_shared_rank(&sh.pub_best, q));
-    const uint32_t* l = cl.map_shared_rank(&sh.pub_low[0], q);
-    low[0] = min(low[0], l[0]);
-    low[1] = min(low[1], l[1]);
+    low = min(low, *cl.map_shared_rank(&sh.pub_low, q));
   }
   Row<T> row;
   row.vecs = vecs;
   row.count = count;
   row.top = row_top;
-  row.m = (double)K::value(row_top);
   row.pow2 = sh.pow2;
   const float T_row = temperature ? temperature[r] : 1.f;
-  row.scale = 1.4426950408889634 / (double)T_row;
+  const float m = K::value(row_top);
+  const double scale = 1.4426950408889634 / (double)T_row;
+  row.c1 = (float)scale;
+  row.c2 = (float)(scale - (double)row.c1);
+  row.mp = __fmul_rn(m, row.c1);
+  row.me = fmaf(m, row.c1, -row.mp);
+  row.ml = __fmul_rn(m, row.c2);
+  // (a product that overflows, as at temperatures near 0: the largest logit alone has a weight)
+  row.inf = isinf(m) || !(fabsf(row.mp) < 1e37f);
+  row.least = fmaxf(__double2float_ru((double)m - 60.0 / scale), -3.4028234663852886e38f);
   const bool empty = row_top <= K::NONE;
   if (empty || !(T_row > 0.f)) {  // nothing to draw, or greedy: the lowest id of the largest logit
     if (!empty) {
@@ -516,14 +573,39 @@ __global__ void __launch_bounds__(RT, 2)
   // ---- the cuts
   const int k = top_k ? top_k[r] : 0;
   const float tp = top_p ? top_p[r] : 1.f, mp = min_p ? min_p[r] : 0.f;
-  const double floor_w = mp > 0.f ? (double)mp : 0.0;
+  const unsigned long long floor_w = mp > 0.f ? (unsigned long long)ceil(fmin((double)mp, 1.0) * FIX) : 0ull;
   const bool some = k > 0 && k < vocab;
-  // A lower bound of all cuts. ctas * RW warps each hold a token of at least the lowest warp maximum:
-  // with so many of them or fewer the k-th largest is no lower. Without top-p, whose mass counts the
-  // tokens that min-p cuts, min-p is a bound too (a key lower for the rounding of the logarithm).
-  uint32_t bound = some && k <= ctas * RW ? low[0] : 0u;
+  // A lower bound of all cuts: the k-th largest of the quarter warps' maxima (or of the warps', where
+  // they are enough), each of which is a token, is no larger than the k-th largest token, and little
+  // less. Without top-p, whose mass counts the tokens that min-p cuts, min-p is a bound too (a key
+  // lower for the rounding of the logarithm).
+  uint32_t bound = 0u;
+  if (some && k <= 4 * RW * ctas) {
+    const int pool = k <= RW * ctas ? RW * ctas : 4 * RW * ctas;
+    uint32_t mine = 0u;
+    if (tid < pool) {
+      const uint32_t* theirs = cl.map_shared_rank(&sh.pub_tops[0], tid / (pool / ctas));
+      const int at = tid % (pool / ctas);
+      if (pool == RW * ctas)
+        mine = max(max(theirs[4 * at], theirs[4 * at + 1]), max(theirs[4 * at + 2], theirs[4 * at + 3]));
+      else
+        mine = theirs[at];
+      sh.tops[tid] = mine;
+    }
+    __syncthreads();
+    if (tid < pool) {
+      int at_least = 0;
+      for (int i = 0; i < pool; i += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(&sh.tops[i]);
+        at_least += (x.x >= mine) + (x.y >= mine) + (x.z >= mine) + (x.w >= mine);
+      }
+      if (at_least >= k) atomicMax(&sh.bound, mine);
+    }
+    __syncthreads();
+    bound = sh.bound;
+  }
   if (mp > 0.f && !(tp < 1.f)) {
-    const double x0 = row.m + (double)T_row * log(fmin(floor_w, 1.0));
+    const double x0 = (double)m + (double)T_row * log(fmin((double)mp, 1.0));
     const uint32_t f = x0 > -3.0e38 ? K::key_of(__double2float_rd(x0)) : 0u;
     bound = max(bound, min(f > 0u ? f - 1u : 0u, row_top));
   }
@@ -547,16 +629,19 @@ __global__ void __launch_bounds__(RT, 2)
   if (mp > 1.f) {
     cut = select_cut<T, false>(cl, sh, row, row_top, row_top, 1ull);
   } else {
-    if (some) {  // (the threads' maxima bound the k-th largest as the warps' do)
-      uint32_t lo = k <= ctas * RW ? low[0] : k <= ctas * RT ? low[1] : 0u;
-      lo = max(lo, K::NONE + 1u);
+    if (some) {  // (the threads' maxima bound the k-th largest too)
+      const uint32_t lo = max(max(bound, k <= ctas * RT ? low : 0u), K::NONE + 1u);
       cut = select_cut<T, false>(cl, sh, row, lo, row_top, (unsigned long long)k);
     }
     if (tp < 1.f) {
       unsigned long long z = 0;
-      row.above(cut.key, [&](int, uint32_t key) {
-        if (key > cut.key || !cut.ties) z += row.fixed(key);
-      });
+      if (cut.ties) {
+        row.above(cut.key, [&](int, uint32_t key) {
+          if (key > cut.key) z += row.fixed(key);
+        });
+      } else {
+        for (int v = tid; v < count; v += RT) z += row.vector_mass(vecs[v]);
+      }
       z = cluster_sum(cl, sh, z);
       if (cut.ties) z += (unsigned long long)cut.keep * row.fixed(cut.key);
       const double edge = ceil((double)fmaxf(tp, 0.f) * (double)z);
@@ -565,7 +650,7 @@ __global__ void __launch_bounds__(RT, 2)
       // at or above w0 (taken a little lower for the rounding of the logarithm)
       const double w0 = (1.0 - (double)fmaxf(tp, 0.f)) * ((double)z / FIX) / vocab * 0.999;
       uint32_t lo = cut.key;
-      const double x0 = row.m + (double)T_row * log(w0);
+      const double x0 = (double)m + (double)T_row * log(w0);
       if (x0 > -3.0e38) {
         const uint32_t f = K::key_of(__double2float_rd(x0));
         lo = max(lo, min(f > 0u ? f - 1u : 0u, row_top));
@@ -608,8 +693,8 @@ __global__ void __launch_bounds__(RT, 2)
       const uint32_t key = K::at(x, j);
       if (key < cut.key) continue;
       if (key == cut.key && partial && ranked++ >= cut.keep) continue;
-      const double w = row.weight(key);
-      if (w >= fmin(floor_w, 1.0)) each(j, __double2ull_rn(w * FIX));
+      const unsigned long long w = row.fixed(key);
+      if (w >= floor_w) each(j, w);
     }
   };
   // ties in the lanes before this one's, and in all of them (only where the cut divides its ties)
@@ -636,10 +721,15 @@ __global__ void __launch_bounds__(RT, 2)
   } none;
 #pragma unroll
   for (int j = 0; j < PER; ++j) none.e[j] = K::PAD;
+  const bool whole = !cut.ties && floor_w == 0ull;  // every token is kept
   unsigned long long sum = 0;
   uint32_t before_ties = tie_base;
   for (int b = begin; b < end; b += 32) {
     const uint4 x = b + lane < end ? vecs[b + lane] : none.v;
+    if (whole) {
+      sum += row.vector_mass(x);
+      continue;
+    }
     const uint32_t ranked = rank_of(x, before_ties);
     kept(x, ranked, [&](int, unsigned long long w) { sum += w; });
   }
@@ -700,15 +790,18 @@ template <typename T>
 int launch_sample_rows(const void* logits, int rows, int vocab, long long row_stride, const float* temperature,
                        const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
                        int32_t* tokens, float* probs, int* status, cudaStream_t stream) {
-  int ctas = 1;
-  // about 8,192 tokens a CTA: below that the cluster's barriers cost more than the shorter slices save
-  while (ctas < MAX_CLUSTER && vocab > 8192 * ctas) ctas *= 2;
+  int dev = 0, sms = 148, ctas = 1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NE_ERR_CUDA;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // Slices of up to 80 KB, two CTAs an SM: the barriers of a larger cluster cost more than its shorter
+  // slices save (measured, 320 rows of 151,936 bf16, top-k 20: 2 / 4 / 8 CTAs 97 / 79 / 123 us). Few rows
+  // leave SMs idle, and slices above 8,192 tokens are halved then.
+  while (ctas < MAX_CLUSTER && (size_t)vocab * sizeof(T) > (80u << 10) * ctas) ctas *= 2;
+  while (ctas < MAX_CLUSTER && vocab > 8192 * ctas && 2LL * rows * ctas <= sms) ctas *= 2;
   const int slice = (vocab + ctas - 1) / ctas;
   const size_t smem = ((size_t)slice * sizeof(T) + 47) / 16 * 16;  // (a padded vector at either end)
   if (smem > MAX_SLICE_BYTES) return NE_ERR_UNSUPPORTED;
   static bool done[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NE_ERR_CUDA;
   if (!done[dev]) {
     if (cudaFuncSetAttribute(sample_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)MAX_SLICE_BYTES) != cudaSuccess)
