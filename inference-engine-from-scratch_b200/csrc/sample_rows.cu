@@ -29,12 +29,25 @@ constexpr int RT = 512;               // threads per CTA
 constexpr int RW = RT / 32;
 constexpr int BINS = 1024;
 constexpr int MOST = 2048;            // tokens of a list
+constexpr int BANDS = 12;
+constexpr int MOST_CHUNKS = 18;       // (MAX_SLICE_BYTES over 16 warps of 32 vectors)
 constexpr int MAX_CLUSTER = 8;
 constexpr unsigned ALL = 0xFFFFFFFFu;
+// 2^(31 + i / 64), rounded
+__device__ const uint32_t POW2[64] = {
+    2147483648u, 2170868212u, 2194507417u, 2218404036u, 2242560872u, 2266980759u, 2291666561u, 2316621173u,
+    2341847524u, 2367348571u, 2393127307u, 2419186755u, 2445529972u, 2472160047u, 2499080105u, 2526293303u,
+    2553802834u, 2581611923u, 2609723834u, 2638141863u, 2666869345u, 2695909648u, 2725266179u, 2754942382u,
+    2784941738u, 2815267765u, 2845924021u, 2876914102u, 2908241642u, 2939910317u, 2971923842u, 3004285971u,
+    3037000500u, 3070071267u, 3103502151u, 3137297074u, 3171459999u, 3205994934u, 3240905930u, 3276197082u,
+    3311872529u, 3347936457u, 3384393094u, 3421246719u, 3458501653u, 3496162267u, 3534232978u, 3572718252u,
+    3611622603u, 3650950594u, 3690706840u, 3730896002u, 3771522796u, 3812591987u, 3854108391u, 3896076880u,
+    3938502376u, 3981389855u, 4024744348u, 4068570940u, 4112874773u, 4157661043u, 4202935003u, 4248701965u};
 constexpr double FIX = 35184372088832.0;          // 2^45
 constexpr unsigned long long ONE = 1ull << 45;    // a weight of 1
 constexpr int MAX_VOCAB = 1 << 18;        // 262,144 weights of at most 1 sum to at most 2^63
 constexpr size_t MAX_SLICE_BYTES = 132 << 10;  // MAX_VOCAB / MAX_CLUSTER tokens in fp32, and a padded vector
+static_assert((MAX_SLICE_BYTES / 16 + RW - 1) / RW <= 32 * MOST_CHUNKS, "a warp's chunks");
 
 // Ordered key of a logit, in the low bits: 16 for bf16, 32 for fp32. NaN and -inf: never drawn.
 // A vector is 16 bytes of a row; ``top`` is its largest logit (NaN aside).
@@ -113,12 +126,15 @@ struct Shared {
   union {
     Bins bins[2];
     List list;
+    float column[BANDS][RT];  // a thread's sums of the weights in (4^-(b + 1), 4^-b]
   };
+  unsigned long long chunk[RW][MOST_CHUNKS];  // kept mass of a warp's part, 32 vectors at a time
   unsigned long long red64[RW];
   uint32_t red32[RW];
   uint2 pow2[64];  // 2^(31 + i / 64) in 32 bits (2^32 - 1 at most), and an eighth of it as a float
   // published to the cluster
-  unsigned long long pub_sum;
+  unsigned long long pub_sum[3], pub_above;
+  float pub_band[BANDS];
   uint32_t pub_best, pub_low, pub_ties, pub_listed, bound;
   uint32_t pub_tops[4 * RW];               // the largest key of each quarter warp
   alignas(16) uint32_t tops[4 * RW * MAX_CLUSTER];  // (the cluster's)
@@ -137,12 +153,33 @@ struct Cut {
   uint32_t key, keep, ties;
 };
 
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  return (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 template <typename T>
 struct Row {
   const uint4* vecs;   // this CTA's slice: vector v holds tokens PER v .. of it, padded with -inf
   int count;           // its vectors
   uint32_t top;        // the row's largest key
-  bool inf;            // it is infinite
+  bool inf;            // it alone has a weight
+  bool careful;        // (a temperature so high that masked logits have to be told apart by their keys)
   float least;         // a logit whose weight is 2^-60
   float c1, c2;        // log2(e) / temperature = c1 + c2
   float mp, me, ml;    // the largest logit times c1 (its product, and the rounding error of that) and c2
@@ -154,36 +191,61 @@ struct Row {
   // that t is off by less than 2^-30; the weight by about 2e-9 of itself, each logit's differently.
   // (The same in fp64 took a pass over a row from 6 to 25 us.) A logit below ``least``, -inf or NaN
   // weighs 2^-60, which is 0.
-  __device__ __forceinline__ unsigned long long power(float logit) const {
-    const float x = fmaxf(logit, least);
-    // (the rounded operations by name: none may be contracted with another)
-    const float p = __fmul_rn(x, c1), e = fmaf(x, c1, -p);    // x c1 = p + e
-    const float s = __fsub_rn(p, mp), z = __fsub_rn(s, p);    // p - mp = s + err
-    const float err = __fsub_rn(__fsub_rn(p, __fsub_rn(s, z)), __fadd_rn(mp, z));
-    const float low = err + (__fsub_rn(e, me) + fmaf(x, c2, -ml));
+  __device__ __forceinline__ void power2(float logit_a, float logit_b, unsigned long long& wa, unsigned long long& wb,
+                                         int* band = nullptr, float* approx = nullptr) const {
+    constexpr uint64_t MINUS = 0xBF800000BF800000ull;         // (-1, -1): a - b as fma(b, -1, a), one rounding
+    const uint64_t x = pair(fmaxf(logit_a, least), fmaxf(logit_b, least)), c = pair(c1, c1), m2 = pair(mp, mp);
+    const uint64_t p = mul2(x, c), e = fma2(x, c, mul2(p, MINUS));  // x c1 = p + e
+    const uint64_t s = fma2(m2, MINUS, p), z = fma2(p, MINUS, s);   // p - mp = s + err
+    const uint64_t err = fma2(add2(m2, z), MINUS, fma2(fma2(z, MINUS, s), MINUS, p));
+    const uint64_t low = add2(err, add2(fma2(pair(me, me), MINUS, e), fma2(x, pair(c2, c2), pair(-ml, -ml))));
     constexpr float MAGIC = 196608.f;                         // 1.5 x 2^17: s rounded to 1 / 64
-    const float u = __fadd_rn(s, MAGIC);
-    const int n = __float_as_int(u) - 0x48400000;
-    const float r = __fsub_rn(s, __fsub_rn(u, MAGIC)) + low;
-    float y = fmaf(r, 0.009618129f, 0.05550411f);
-    y = fmaf(y, r, 0.24022651f);
-    y = fmaf(y, r, 0.69314718f) * r;                          // 2^r - 1
-    const uint2 t = pow2[n & 63];                             // 2^(31 + n / 64), and an eighth as a float
+    const uint64_t u = add2(s, pair(MAGIC, MAGIC));
+    const uint64_t r = add2(fma2(add2(u, pair(-MAGIC, -MAGIC)), MINUS, s), low);
+    uint64_t y = fma2(r, pair(0.009618129f, 0.009618129f), pair(0.05550411f, 0.05550411f));
+    y = fma2(y, r, pair(0.24022651f, 0.24022651f));
+    y = mul2(fma2(y, r, pair(0.69314718f, 0.69314718f)), r);  // 2^r - 1
+    const int na = (int)(uint32_t)u - 0x48400000, nb = (int)(uint32_t)(u >> 32) - 0x48400000;
+    const uint2 ta = pow2[na & 63], tb = pow2[nb & 63];       // 2^(31 + n / 64), and an eighth as a float
+    const uint64_t t8 = (uint64_t)ta.y | (uint64_t)tb.y << 32;
     // (|y| < 0.0055: the product is below 2^22, where 1.5 x 2^23 rounds it to an integer)
-    const int i = __float_as_int(fmaf(y, __uint_as_float(t.y), 12582912.f)) - 0x4B400000;
-    return ((unsigned long long)(t.x + (uint32_t)(i * 8)) << 14) >> (unsigned)-(n >> 6);
+    const uint64_t i = fma2(y, t8, pair(12582912.f, 12582912.f));
+    const uint32_t va = ta.x + ((uint32_t)i - 0x4B400000u) * 8u, vb = tb.x + ((uint32_t)(i >> 32) - 0x4B400000u) * 8u;
+    wa = ((unsigned long long)va << 14) >> (unsigned)-(na >> 6);
+    wb = ((unsigned long long)vb << 14) >> (unsigned)-(nb >> 6);
+    if (band) {  // for a coarse sum by weight: the band of 4^-b, and the weight times 2^28 in fp32
+      const uint64_t f = fma2(y, t8, t8);
+      band[0] = min(-na >> 7, BANDS - 1);
+      band[1] = min(-nb >> 7, BANDS - 1);
+      approx[0] = __int_as_float((int)(uint32_t)f + (na >> 6) * (1 << 23));
+      approx[1] = __int_as_float((int)(uint32_t)(f >> 32) + (nb >> 6) * (1 << 23));
+    }
+  }
+  __device__ __forceinline__ unsigned long long power(float logit) const {
+    unsigned long long a, b;
+    power2(logit, logit, a, b);
+    return a;
   }
   // (an infinite largest logit: all for it, nothing for the rest)
   __device__ __forceinline__ unsigned long long fixed(uint32_t k) const {
     if (inf) return k == top ? ONE : 0ull;
     return k <= Keys<T>::NONE ? 0ull : power(Keys<T>::value(k));
   }
-  // the mass of all tokens of a vector
-  __device__ __forceinline__ unsigned long long vector_mass(const uint4& v) const {
-    unsigned long long sum = 0;
+  // the masses of a vector's tokens, side by side
+  __device__ __forceinline__ void masses(const uint4& v, unsigned long long (&w)[Keys<T>::PER]) const {
+    if (careful) {
 #pragma unroll
-    for (int j = 0; j < Keys<T>::PER; ++j)
-      sum += inf ? fixed(Keys<T>::at(v, j)) : power(Keys<T>::logit(v, j));
+      for (int j = 0; j < Keys<T>::PER; ++j) w[j] = fixed(Keys<T>::at(v, j));
+    } else {
+#pragma unroll
+      for (int j = 0; j < Keys<T>::PER; j += 2) power2(Keys<T>::logit(v, j), Keys<T>::logit(v, j + 1), w[j], w[j + 1]);
+    }
+  }
+  __device__ __forceinline__ unsigned long long vector_mass(const uint4& v) const {
+    unsigned long long w[Keys<T>::PER], sum = 0;
+    masses(v, w);
+#pragma unroll
+    for (int j = 0; j < Keys<T>::PER; ++j) sum += w[j];
     return sum;
   }
 
@@ -210,7 +272,8 @@ __device__ __forceinline__ unsigned long long warp_add(unsigned long long v) {
 }
 
 // Sum over the CTA, then over the cluster; every thread of the cluster gets it.
-__device__ unsigned long long cluster_sum(cg::cluster_group& cl, Shared& sh, unsigned long long v) {
+// Each call of a row has a place of its own (``turn``), so that none is set while another CTA reads it.
+__device__ unsigned long long cluster_sum(cg::cluster_group& cl, Shared& sh, unsigned long long v, int turn) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_add(v);
   if (lane == 0) sh.red64[warp] = v;
@@ -218,22 +281,33 @@ __device__ unsigned long long cluster_sum(cg::cluster_group& cl, Shared& sh, uns
   if (threadIdx.x == 0) {
     unsigned long long t = 0;
     for (int w = 0; w < RW; ++w) t += sh.red64[w];
-    sh.pub_sum = t;
+    sh.pub_sum[turn] = t;
   }
   cl.sync();
   unsigned long long total = 0;
-  for (unsigned r = 0; r < cl.num_blocks(); ++r) total += *cl.map_shared_rank(&sh.pub_sum, r);
-  cl.sync();  // read everywhere before the next use
+  for (unsigned r = 0; r < cl.num_blocks(); ++r) total += *cl.map_shared_rank(&sh.pub_sum[turn], r);
   return total;
 }
 
 // The cut at which the tokens with larger keys, and some of the ties, first reach ``limit``: a count
-// (MASS false) or a mass in fixed point. Only keys in [lo, hi] are looked at; the tokens above hi
-// are none, and those in [lo, hi] reach the limit (or the cut is the lowest key present).
+// (MASS false) or a mass in fixed point. It is looked for in [lo, hi] (a mass above hi is added up);
+// with no ties it is not there. At the bottom of all cuts (``last``) it is the lowest key present
+// where the limit is not reached.
 template <typename T, bool MASS>
 __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, uint32_t lo, uint32_t hi,
-                          unsigned long long limit) {
+                          unsigned long long limit, bool last = true) {
   unsigned long long above = 0;
+  bool first = true;
+  // The first pass of masses cuts a wide range evenly by the logits: keys are even by their logarithm,
+  // and put most of a row into a few bins around the bulk, whose atomics then queue (58,000 cycles a
+  // pass). Later passes take the tokens of the chosen ``slot`` by the same arithmetic.
+  const float x_hi = Keys<T>::value(hi), x_lo = Keys<T>::value(lo);
+  const float per = (float)BINS / (x_hi - x_lo);
+  const bool even = MASS && hi - lo >= BINS && per > 0.f && per < 1e30f;
+  auto slot_of = [&](uint32_t k) -> int {
+    return BINS - 1 - min(BINS - 1, (int)((x_hi - Keys<T>::value(k)) * per));
+  };
+  int slot = -1;
   int buf = 0;
   uint32_t ties = 0;
   for (;;) {
@@ -245,17 +319,45 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
       if (MASS) bins.piece[0][i] = bins.piece[1][i] = bins.piece[2][i] = 0u;
     }
     __syncthreads();
-    row.above(max(lo, Keys<T>::NONE + 1u), [&](int, uint32_t k) {
-      if (k > hi) return;
-      const uint32_t b = (k - lo) >> shift;
-      atomicAdd(&bins.count[b], 1u);
-      if (MASS) {
-        const unsigned long long f = row.fixed(k);
-        atomicAdd(&bins.piece[0][b], (uint32_t)f & 0x7FFFu);
-        atomicAdd(&bins.piece[1][b], (uint32_t)(f >> 15) & 0x7FFFu);
-        atomicAdd(&bins.piece[2][b], (uint32_t)(f >> 30));
+    // (a bin of one key needs no masses: they are its count times the key's)
+    const bool start = MASS && first, pieces = MASS && shift > 0;
+    unsigned long long outer = 0;
+    const uint32_t least = max(lo, Keys<T>::NONE + 1u);
+    const float least_value = Keys<T>::value(least), hi_value = Keys<T>::value(hi);
+    for (int v = threadIdx.x; v < row.count; v += RT) {
+      const uint4 x = row.vecs[v];
+      const float t = Keys<T>::top(x);
+      if (!(t >= least_value)) continue;
+      unsigned long long f[Keys<T>::PER];
+      if (pieces || (start && t > hi_value)) row.masses(x, f);  // (side by side: one at a time, behind each
+#pragma unroll                                                  // test, took three times as long)
+      for (int j = 0; j < Keys<T>::PER; ++j) {
+        const uint32_t k = Keys<T>::at(x, j);
+        if (k < least) continue;
+        if (k > hi) {
+          if (start) outer += f[j];
+          continue;
+        }
+        if (slot >= 0 && slot_of(k) != slot) continue;
+        const uint32_t b = even && first ? (uint32_t)slot_of(k) : (k - lo) >> shift;
+        atomicAdd(&bins.count[b], 1u);
+        if (pieces) {
+          atomicAdd(&bins.piece[0][b], (uint32_t)f[j] & 0x7FFFu);
+          atomicAdd(&bins.piece[1][b], (uint32_t)(f[j] >> 15) & 0x7FFFu);
+          atomicAdd(&bins.piece[2][b], (uint32_t)(f[j] >> 30));
+        }
       }
-    });
+    }
+    if (start) {
+      outer = warp_add(outer);
+      if ((threadIdx.x & 31) == 0) sh.red64[threadIdx.x >> 5] = outer;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        unsigned long long t = 0;
+        for (int x = 0; x < RW; ++x) t += sh.red64[x];
+        sh.pub_above = t;
+      }
+    }
     cl.sync();
     // every CTA adds the cluster's bins: thread t owns bins 2 t and 2 t + 1
     uint32_t c[2] = {0u, 0u};
@@ -266,7 +368,8 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
       const uint2 rc = reinterpret_cast<const uint2*>(remote->count)[threadIdx.x];
       c[0] += rc.x;
       c[1] += rc.y;
-      if (MASS) {
+      if (start) above += *cl.map_shared_rank(&sh.pub_above, r);
+      if (pieces) {
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
           const uint2 rp = reinterpret_cast<const uint2*>(remote->piece[q])[threadIdx.x];
@@ -274,6 +377,11 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
           w[1] += (unsigned long long)rp.y << (15 * q);
         }
       }
+    }
+    if (MASS && !pieces) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (c[j]) w[j] = c[j] * row.fixed(lo + 2 * threadIdx.x + j);
     }
     const unsigned long long v[2] = {MASS ? w[0] : c[0], MASS ? w[1] : c[1]};
     // mass (or count) of the bins above this thread's: an exclusive suffix sum
@@ -288,7 +396,13 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
     if (threadIdx.x == 0) sh.sel_bin = -1;
     __syncthreads();
     unsigned long long before = above + incl - (v[0] + v[1]);
-    for (int x = warp + 1; x < RW; ++x) before += sh.red64[x];
+    unsigned long long all = 0;
+    for (int x = 0; x < RW; ++x) {
+      const unsigned long long t = sh.red64[x];
+      if (x > warp) before += t;
+      all += t;
+    }
+    if (start && !last && above + all < limit) return Cut{lo, 0u, 0u};
     // the lowest non-empty bin whose tokens start below the limit: each thread offers its own
     int mine = -1;
     unsigned long long mine_before = 0;
@@ -314,13 +428,25 @@ __device__ Cut select_cut(cg::cluster_group& cl, Shared& sh, const Row<T>& row, 
     }
     __syncthreads();
     const int bin = sh.sel_bin;
-    if (bin < 0) break;  // no token in the range (not reached: the largest key starts at 0)
+    if (bin < 0) return Cut{lo, 0u, 0u};  // (the limit lies above hi)
     above = sh.sel_mass;
     ties = sh.sel_count;
+    if (even && first) {
+      // keys that the slot's tokens lie between, with a margin for the slots' arithmetic
+      slot = bin;
+      const float d = (float)(BINS - 1 - bin);
+      const uint32_t a = Keys<T>::key_of(x_hi - (d + 1.01f) / per), z = Keys<T>::key_of(x_hi - (d - 0.01f) / per);
+      lo = max(lo, a > 0u ? a - 1u : 0u);
+      hi = max(lo, min(hi, z + 1u));
+      first = false;
+      buf ^= 1;
+      continue;
+    }
     const uint32_t nlo = lo + ((uint32_t)bin << shift);
     const uint32_t last = nlo + ((1u << shift) - 1u);
     hi = last < nlo ? hi : min(hi, last);
     lo = nlo;
+    first = false;
     buf ^= 1;  // (the other CTAs may still read this buffer)
     if (shift == 0) break;
   }
@@ -479,10 +605,7 @@ __global__ void __launch_bounds__(RT, 2)
   const int r = blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = min(vocab, rank * slice), n = min(vocab, first + slice) - first;
-  if (tid < 64) {
-    const double v = rint(exp2(31.0 + (double)tid * (1.0 / 64.0)));
-    sh.pow2[tid] = make_uint2((uint32_t)v, __float_as_uint((float)(v * 0.125)));
-  }
+  if (tid < 64) sh.pow2[tid] = make_uint2(POW2[tid], __float_as_uint((float)POW2[tid] * 0.125f));
 
   // ---- the slice into shared memory; 16-byte loads from the first aligned logit on. Vector 0 of the
   // slice starts at that boundary's token or before: ``skew`` places of it are padding
@@ -493,11 +616,9 @@ __global__ void __launch_bounds__(RT, 2)
   const int count = n > 0 ? (skew + n + PER - 1) / PER : 0;
   const uint4* vsrc = reinterpret_cast<const uint4*>(src - skew);
   float top = -INFINITY;
-#pragma unroll 4
   for (int v = tid; v < count; v += RT) {
-    uint4 x;
     if ((v > 0 || skew == 0) && (v + 1) * PER <= skew + n) {
-      x = vsrc[v];
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(vecs + v)), "l"(vsrc + v) : "memory");
     } else {  // the first or last vector, in part
       union {
         uint4 v;
@@ -508,11 +629,11 @@ __global__ void __launch_bounds__(RT, 2)
         const int i = v * PER + j - skew;
         part.e[j] = i >= 0 && i < n ? src[i] : K::PAD;
       }
-      x = part.v;
+      vecs[v] = part.v;
     }
-    vecs[v] = x;
-    top = fmaxf(top, K::top(x));
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // (a thread reads its own vectors until the first barrier)
+  for (int v = tid; v < count; v += RT) top = fmaxf(top, K::top(vecs[v]));
 
   // ---- the row's largest logit, and the largest of each eight lanes' tokens
   uint32_t top_key = K::key_of(top);
@@ -547,15 +668,22 @@ __global__ void __launch_bounds__(RT, 2)
   row.pow2 = sh.pow2;
   const float T_row = temperature ? temperature[r] : 1.f;
   const float m = K::value(row_top);
-  const double scale = 1.4426950408889634 / (double)T_row;
-  row.c1 = (float)scale;
-  row.c2 = (float)(scale - (double)row.c1);
+  constexpr float LOG2E_1 = 1.442695041f, LOG2E_2 = 1.925963e-8f;  // log2(e) in two parts
+  row.c1 = LOG2E_1 / T_row;
+  row.c2 = (fmaf(-row.c1, T_row, LOG2E_1) + LOG2E_2) / T_row;
   row.mp = __fmul_rn(m, row.c1);
   row.me = fmaf(m, row.c1, -row.mp);
   row.ml = __fmul_rn(m, row.c2);
   // (a product that overflows, as at temperatures near 0: the largest logit alone has a weight)
   row.inf = isinf(m) || !(fabsf(row.mp) < 1e37f);
-  row.least = fmaxf(__double2float_ru((double)m - 60.0 / scale), -3.4028234663852886e38f);
+  row.careful = row.inf || T_row > 1e30f;
+  row.least = fmaxf(m - 41.6f * T_row, -3.4028234663852886e38f);  // (60 ln 2: a weight of 2^-60)
+  // the key of a logit that weighs w, or of one a little lighter (the logarithm's error is a bound's)
+  auto key_at = [&](float w) -> uint32_t {
+    const float x = m + T_row * (logf(w) - 1e-3f);
+    const uint32_t f = x > -3.0e38f ? K::key_of(x) : 0u;
+    return min(f > 0u ? f - 1u : 0u, row_top);
+  };
   const bool empty = row_top <= K::NONE;
   if (empty || !(T_row > 0.f)) {  // nothing to draw, or greedy: the lowest id of the largest logit
     if (!empty) {
@@ -605,14 +733,12 @@ __global__ void __launch_bounds__(RT, 2)
     bound = sh.bound;
   }
   if (mp > 0.f && !(tp < 1.f)) {
-    const double x0 = (double)m + (double)T_row * log(fmin((double)mp, 1.0));
-    const uint32_t f = x0 > -3.0e38 ? K::key_of(__double2float_rd(x0)) : 0u;
-    bound = max(bound, min(f > 0u ? f - 1u : 0u, row_top));
+    bound = max(bound, key_at(fminf(mp, 1.f)));
   }
   if (bound > K::NONE) {
     uint32_t have = 0;
     row.above(bound, [&](int, uint32_t) { ++have; });
-    const unsigned long long n_list = cluster_sum(cl, sh, have);
+    const unsigned long long n_list = cluster_sum(cl, sh, have, 0);
     if (n_list <= MOST) {
       row.above(bound, [&](int i, uint32_t key) {
         const uint32_t at = atomicAdd(cl.map_shared_rank(&sh.pub_listed, 0), 1u);
@@ -635,27 +761,70 @@ __global__ void __launch_bounds__(RT, 2)
     }
     if (tp < 1.f) {
       unsigned long long z = 0;
+      // with top-k the few tokens that are left; else every token, and where their mass lies by bands of
+      // the weight: a column of sums a thread, in shared memory, without atomics
+      const bool banded = !cut.ties && !row.careful;
       if (cut.ties) {
         row.above(cut.key, [&](int, uint32_t key) {
           if (key > cut.key) z += row.fixed(key);
         });
-      } else {
+      } else if (!banded) {
         for (int v = tid; v < count; v += RT) z += row.vector_mass(vecs[v]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < BANDS; ++x) sh.column[x][tid] = 0.f;
+        for (int v = tid; v < count; v += RT) {
+          const uint4 x = vecs[v];
+          int band[PER];
+          float approx[PER];
+#pragma unroll
+          for (int j = 0; j < PER; j += 2) {
+            unsigned long long a, b;
+            row.power2(K::logit(x, j), K::logit(x, j + 1), a, b, &band[j], &approx[j]);
+            z += a + b;
+          }
+#pragma unroll
+          for (int j = 0; j < PER; ++j) sh.column[band[j]][tid] += approx[j];
+        }
+        __syncthreads();
+        if (warp < BANDS) {
+          float t = 0.f;
+#pragma unroll
+          for (int i = 0; i < RT / 32; ++i) t += sh.column[warp][i * 32 + lane];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(ALL, t, o);
+          if (lane == 0) sh.pub_band[warp] = t;
+        }
       }
-      z = cluster_sum(cl, sh, z);
+      z = cluster_sum(cl, sh, z, 1);
       if (cut.ties) z += (unsigned long long)cut.keep * row.fixed(cut.key);
       const double edge = ceil((double)fmaxf(tp, 0.f) * (double)z);
       const unsigned long long limit = edge < 1.0 ? 1ull : (unsigned long long)edge;
-      // tokens below w0 = (1 - top_p) z / vocab hold less than (1 - top_p) z together: the cut is
-      // at or above w0 (taken a little lower for the rounding of the logarithm)
-      const double w0 = (1.0 - (double)fmaxf(tp, 0.f)) * ((double)z / FIX) / vocab * 0.999;
-      uint32_t lo = cut.key;
-      const double x0 = (double)m + (double)T_row * log(w0);
-      if (x0 > -3.0e38) {
-        const uint32_t f = K::key_of(__double2float_rd(x0));
-        lo = max(lo, min(f > 0u ? f - 1u : 0u, row_top));
+      // tokens below w0 = (1 - top_p) z / vocab hold less than (1 - top_p) z together: the cut is at or
+      // above w0
+      const float w0 = (1.f - fmaxf(tp, 0.f)) * ((float)((double)z / FIX) / vocab * 0.999f);
+      const uint32_t lo = max(cut.key, w0 > 0.f ? key_at(w0) : 0u);
+      Cut found{lo, 0u, 0u};
+      if (banded) {
+        // the bands whose running sum passes the limit, give or take the sums' error
+        const float want = (float)((double)limit / FIX) * 268435456.f;  // (the bands' weights are times 2^28)
+        int b0 = BANDS, b1 = BANDS;
+        float run = 0.f;
+        for (int x = 0; x < BANDS; ++x) {
+          for (int q = 0; q < ctas; ++q) run += cl.map_shared_rank(&sh.pub_band[0], q)[x];
+          if (b0 == BANDS && run >= want * 0.999f) b0 = x;
+          if (b1 == BANDS && run >= want * 1.001f) b1 = x;
+        }
+        if (b1 < BANDS - 1) {
+          const float above = b0 > 0 ? m + T_row * (-1.3862944f * b0 + 0.02f) : m;  // (a band is rounded by 1 / 128)
+          const uint32_t band_hi = b0 > 0 ? min(K::key_of(above) + 1u, row_top) : row_top;
+          const uint32_t band_lo = max(lo, key_at(exp2f(-2.f * b1 - 2.02f)));
+          if (band_lo <= band_hi) found = select_cut<T, true>(cl, sh, row, band_lo, band_hi, limit, band_lo == lo);
+          if (!found.ties) cl.sync();  // (not there after all: look everywhere)
+        }
       }
-      cut = select_cut<T, true>(cl, sh, row, lo, row_top, limit);
+      if (!found.ties) found = select_cut<T, true>(cl, sh, row, lo, row_top, limit);
+      cut = found;
     }
   }
   const bool partial = cut.ties != 0u && cut.keep < cut.ties;  // the cut divides its ties
@@ -688,13 +857,14 @@ __global__ void __launch_bounds__(RT, 2)
   // the kept mass of a lane's vector (``ranked``: ties before it); each(j, mass) in id order
   auto kept = [&](const uint4& x, uint32_t ranked, auto&& each) {
     if (!(K::top(x) >= least)) return;
+    unsigned long long w[PER];
+    row.masses(x, w);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const uint32_t key = K::at(x, j);
       if (key < cut.key) continue;
       if (key == cut.key && partial && ranked++ >= cut.keep) continue;
-      const unsigned long long w = row.fixed(key);
-      if (w >= floor_w) each(j, w);
+      if (w[j] >= floor_w) each(j, w[j]);
     }
   };
   // ties in the lanes before this one's, and in all of them (only where the cut divides its ties)
@@ -726,24 +896,27 @@ __global__ void __launch_bounds__(RT, 2)
   uint32_t before_ties = tie_base;
   for (int b = begin; b < end; b += 32) {
     const uint4 x = b + lane < end ? vecs[b + lane] : none.v;
+    unsigned long long part = 0;
     if (whole) {
-      sum += row.vector_mass(x);
-      continue;
+      part = row.vector_mass(x);
+    } else {
+      const uint32_t ranked = rank_of(x, before_ties);
+      kept(x, ranked, [&](int, unsigned long long w) { part += w; });
     }
-    const uint32_t ranked = rank_of(x, before_ties);
-    kept(x, ranked, [&](int, unsigned long long w) { sum += w; });
+    part = warp_add(part);
+    if (lane == 0) sh.chunk[warp][(b - begin) >> 5] = part;
+    sum += part;
   }
-  sum = warp_add(sum);
   __syncthreads();
   if (lane == 0) sh.red64[warp] = sum;
   __syncthreads();
   unsigned long long mine = 0;
   for (int w = 0; w < RW; ++w) mine += sh.red64[w];
-  if (tid == 0) sh.pub_sum = mine;
+  if (tid == 0) sh.pub_sum[2] = mine;
   cl.sync();
   unsigned long long total = 0, before = 0;
   for (int q = 0; q < ctas; ++q) {
-    const unsigned long long t = *cl.map_shared_rank(&sh.pub_sum, q);
+    const unsigned long long t = *cl.map_shared_rank(&sh.pub_sum[2], q);
     if (q < rank) before += t;
     total += t;
   }
@@ -755,8 +928,13 @@ __global__ void __launch_bounds__(RT, 2)
     before_ties = tie_base;
     unsigned long long run = before;
     for (int b = begin; b < end; b += 32) {
+      const unsigned long long part = sh.chunk[warp][(b - begin) >> 5];
       const uint4 x = b + lane < end ? vecs[b + lane] : none.v;
       const uint32_t ranked = rank_of(x, before_ties);
+      if (run + part <= target) {
+        run += part;
+        continue;
+      }
       unsigned long long w = 0;
       kept(x, ranked, [&](int, unsigned long long f) { w += f; });
       unsigned long long incl = w;
