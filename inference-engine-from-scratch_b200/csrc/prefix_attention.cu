@@ -490,7 +490,9 @@ __global__ void __launch_bounds__(32 * NW * NT, NT == 2 ? 2 : NW == 8 ? 1 : NW =
 }
 
 // ---------------------------------------------------------------- prefixes: the tensor-core kernel
-constexpr int PRE_THREADS = 384;           // two softmax warpgroups; a load warp, two MMA warps, one idle
+// two softmax warpgroups; a load warp, two MMA warps, one idle; for an int8 pool four warps that load and
+// convert (which then run with 88 registers and leave the softmax 168: 512 x 128 at launch)
+constexpr int pre_threads(bool int8) { return int8 ? 512 : 384; }
 constexpr int SLOT_BYTES = TILE * D * 2;   // one K or V tile: two halves of 64 dimensions, rows of 128 B
 constexpr int RING = 4;
 constexpr int HALF = TILE / 2;             // keys of a softmax step
@@ -512,6 +514,8 @@ struct alignas(16) PreShared {
   uint32_t tmem;
   volatile int abort_flag;
   uint32_t valid[RING];                    // valid blocks of the tile in a slot
+  // int8: K scales (times log2(e) / sqrt(128)) and V scales of the tile whose V is in slot 1 or 3
+  alignas(16) float scale[2][2][TILE];
 };
 constexpr size_t PRE_SMEM = 1024 + 2 * SLOT_BYTES + RING * SLOT_BYTES + sizeof(PrePlan) + sizeof(PreShared);
 static_assert(PRE_SMEM <= 232448, "shared memory of one CTA");
@@ -589,6 +593,11 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -690,10 +699,13 @@ struct Walk {
   }
 };
 
-__global__ void __launch_bounds__(PRE_THREADS, 1)
+template <bool INT8>
+__global__ void __launch_bounds__(pre_threads(INT8), 1)
     prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                  const __nv_bfloat16* __restrict__ q, ne_rows rows, ne_prefix_groups groups, int nh, int nkv,
-                  long long num_cache_slots, Parts parts, int* status) {
+                  const int8_t* __restrict__ kc, const int8_t* __restrict__ vc, const __nv_bfloat16* __restrict__ ks,
+                  const __nv_bfloat16* __restrict__ vs, const __nv_bfloat16* __restrict__ q, ne_rows rows,
+                  ne_prefix_groups groups, int nh, int nkv, long long num_cache_slots, Parts parts, int* status) {
+  constexpr int THREADS_P = pre_threads(INT8);
   pdl_wait();
   pdl_trigger();  // (after the wait: own_tokens_kernel relies on it)
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -708,7 +720,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
   // ---- barriers, tensor memory, and the plan
   if (tid == 0) {
     for (int i = 0; i < RING; ++i) {
-      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.full[i], INT8 ? 64 : 1);  // (a tensor load's thread, or the two warps that convert)
       mbar_init(&sh.empty[i], 2);  // a release by each query tile's products
     }
     for (int s = 0; s < 2; ++s) {
@@ -726,21 +738,21 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
     tmem_alloc(&sh.tmem, TMEM_COLS);
     tmem_relinquish();
   }
-  for (int g = tid; g < ng; g += PRE_THREADS) {
+  for (int g = tid; g < ng; g += THREADS_P) {
     plan.vec[g] = 0;          // (rows, until they are summed)
     plan.group_first[g] = 0;  // (members, until their offsets are known)
     plan.blocks[g] = groups.prefix_blocks[g];
   }
-  for (int b = tid; b < (n + 3 & ~3); b += PRE_THREADS) {
+  for (int b = tid; b < (n + 3 & ~3); b += THREADS_P) {
     const Entry e = b < n ? entry_of(rows, groups, b, nullptr) : Entry{0, 0, -1};  // (own_tokens_kernel reports)
     plan.start[b] = e.start;
     plan.key[b] = e.group >= 0 ? (uint32_t)e.rows << 12 | (uint32_t)(e.group + 1) : 0u;
   }
   __syncthreads();
-  int rank[(MAX_SEQS + PRE_THREADS - 1) / PRE_THREADS];  // members of the group before the entry
+  int rank[(MAX_SEQS + THREADS_P - 1) / THREADS_P];  // members of the group before the entry
 #pragma unroll
-  for (int i = 0; i < (MAX_SEQS + PRE_THREADS - 1) / PRE_THREADS; ++i) {
-    const int b = tid + i * PRE_THREADS;
+  for (int i = 0; i < (MAX_SEQS + THREADS_P - 1) / THREADS_P; ++i) {
+    const int b = tid + i * THREADS_P;
     rank[i] = 0;
     const uint32_t key = b < n ? plan.key[b] : 0u;
     if (key == 0u) continue;
@@ -811,8 +823,8 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
   tc_fence_before();
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < (MAX_SEQS + PRE_THREADS - 1) / PRE_THREADS; ++i) {
-    const int b = tid + i * PRE_THREADS;
+  for (int i = 0; i < (MAX_SEQS + THREADS_P - 1) / THREADS_P; ++i) {
+    const int b = tid + i * THREADS_P;
     if (b < n && plan.key[b]) plan.member[plan.group_first[(plan.key[b] & 0xFFFu) - 1] + rank[i]] = (short)b;
   }
   __syncthreads();
@@ -822,6 +834,10 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
   Walk walk(&plan, groups, nkv, G, per);
   Segment sg;
 
+  if (INT8) {
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
   if (warp < 8) {
     // ------------------------------------------------------------ softmax of query tile s, a row per thread
     const int s = warp >> 2, row = tid & 127;
@@ -882,6 +898,16 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
         ok = ok && mbar_wait(&sh.full[v_at % RING], (v_at / RING) & 1u, &sh.abort_flag, status);
         const uint32_t valid = sh.valid[v_at % RING] >> (4 * half) & 0xFu;
         tmem_ld_wait();
+        const float* scale_k = sh.scale[(v_at % RING) >> 1][0] + HALF * half;
+        const float* scale_v = sh.scale[(v_at % RING) >> 1][1] + HALF * half;
+        if (INT8) {
+#pragma unroll
+          for (int c = 0; c < HALF; c += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(scale_k + c);
+            unpack2(mul2(pack2(x[c], x[c + 1]), pack2(k4.x, k4.y)), x[c], x[c + 1]);
+            unpack2(mul2(pack2(x[c + 2], x[c + 3]), pack2(k4.z, k4.w)), x[c + 2], x[c + 3]);
+          }
+        }
         if (valid != 0xFu) {
 #pragma unroll
           for (int c = 0; c < HALF; ++c)
@@ -897,7 +923,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx[i] = max2(mx[i], x[56 + i]);
         const float top =
-            max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max2(mx[6], mx[7])) * SCALE_LOG2;
+            max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max2(mx[6], mx[7])) * (INT8 ? 1.f : SCALE_LOG2);
         const bool odd = __any_sync(ALL, !(fabsf(top) < INFINITY));  // NaN or infinite scores among them
         // the reference moves only when the scores pass it by 2^8 (the sums stay far inside fp32)
         if (__any_sync(ALL, !(top <= ref + RESCALE))) {
@@ -927,7 +953,8 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < HALF / 2; ++i) {
             float a, b;
-            const uint64_t t2 = fma2(pack2(x[2 * i], x[2 * i + 1]), scale2, base2);
+            const uint64_t x2 = pack2(x[2 * i], x[2 * i + 1]);
+            const uint64_t t2 = INT8 ? add2(x2, base2) : fma2(x2, scale2, base2);  // (int8: scaled already)
             if (all || i % 8 >= POLY_PAIRS) {
               unpack2(t2, a, b);
               a = ex2(a);
@@ -936,6 +963,10 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
               ex2_poly(t2, a, b);
             }
             sum[i & 1] = add2(sum[i & 1], pack2(a, b));
+            if (INT8) {
+              const float2 v2 = *reinterpret_cast<const float2*>(scale_v + 2 * i);
+              unpack2(mul2(pack2(a, b), pack2(v2.x, v2.y)), a, b);
+            }
             p[i] = pack_bf16(a, b);
           }
         };
@@ -991,7 +1022,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
         parts.pre_l[at] = l;
       }
     }
-  } else if (warp == 8 && elect_one()) {
+  } else if (!INT8 && warp == 8 && elect_one()) {
     // ------------------------------------------------------------ loads, issued by one thread
     uint32_t load = 0;  // ring slots filled
     bool ok = true;
@@ -1118,6 +1149,79 @@ __global__ void __launch_bounds__(PRE_THREADS, 1)
       base += 2 * tiles;
     }
   }
+  else if (INT8 && warp >= 12) {
+    // ------------------------------------------------------------ int8 loads: two warps for K, two for V
+    // A tile is 1024 pieces of 16 integers: thread t takes pieces t + 64 i, all loads issued before the
+    // slot is free, and writes each as bf16 (exact) where a tensor load would have put it.
+    const int is_v = (warp - 12) >> 1, t64 = tid & 63, ch = t64 & 7;
+    const int8_t* pool = is_v ? vc : kc;
+    uint32_t tile = 0;
+    bool ok = true;
+    while (ok && walk.next(sg)) {
+      const int blocks = plan.blocks[sg.group];
+      const int32_t* table = table_of(rows, plan.member[plan.group_first[sg.group]]);
+      for (int t = sg.t0; ok && t < sg.t1; ++t, ++tile) {
+        const uint32_t load = 2 * tile + is_v;
+        const int slot = load % RING;
+        uint32_t mask = 0;
+        uint4 x[16];
+        float scale[4];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const int kb = t * 8 + b;
+          long long id = kb < blocks ? table[kb] : -1;
+          if (id < 0 || (id + 1) * 16 > num_cache_slots - 1) {
+            if (kb < blocks && t64 == 0) report(status, NE_DEV_BAD_SLOT);
+            id = -1;
+          }
+          mask |= (id >= 0 ? 1u : 0u) << b;
+#pragma unroll
+          for (int i = 2 * b; i < 2 * b + 2; ++i) {
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (id >= 0)
+              x[i] = *reinterpret_cast<const uint4*>(
+                  pool + ((id * 16 + 8 * (i & 1) + (t64 >> 3)) * nkv + sg.h) * (long long)D + 16 * ch);
+          }
+          // the scales of keys 2 t64 and 2 t64 + 1
+          if (is_v && t64 >> 3 == b) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const long long at = (id * 16 + ((2 * t64 + i) & 15)) * nkv + sg.h;
+              scale[i] = id >= 0 ? __bfloat162float(ks[at]) * SCALE_LOG2 : 0.f;
+              scale[2 + i] = id >= 0 ? __bfloat162float(vs[at]) : 0.f;
+            }
+          }
+        }
+        if (load >= RING) {
+          ok = mbar_wait(&sh.empty[slot], (load / RING - 1) & 1u, &sh.abort_flag, status);
+          ok = __all_sync(ALL, ok);
+          if (!ok) break;
+        }
+        uint8_t* dst = ring + slot * SLOT_BYTES;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = 8 * i + (t64 >> 3);
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            o[2 * k] = dq_pair(w[k], 0x4140u, 0x3F803F80u);
+            o[2 * k + 1] = dq_pair(w[k], 0x4342u, 0x3F803F80u);
+          }
+          uint8_t* row = dst + (ch >> 2) * (SLOT_BYTES / 2) + key * 128;
+          *reinterpret_cast<uint4*>(row + (((2 * ch & 7) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(row + (((2 * ch + 1 & 7) ^ (key & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        if (is_v) {
+          *reinterpret_cast<float2*>(&sh.scale[slot >> 1][0][2 * t64]) = make_float2(scale[0], scale[1]);
+          *reinterpret_cast<float2*>(&sh.scale[slot >> 1][1][2 * t64]) = make_float2(scale[2], scale[3]);
+        }
+        if (t64 == 0) sh.valid[slot] = mask;
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.full[slot]);
+      }
+    }
+  }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -1189,18 +1293,21 @@ int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const vo
       ((long long)rows.max_rows * nh / TILE + 2LL * groups.num_groups * nkv + 2) * (groups.max_prefix_blocks / 8 + 1) >=
           (1 << 28))
     return NE_ERR_UNSUPPORTED;
-  if (kv_int8 || groups.max_prefix_blocks == 0) groups.num_groups = 0;
+  if (groups.max_prefix_blocks == 0) groups.num_groups = 0;
   auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
   const Parts parts{f(l.own_o), f(l.own_m), f(l.own_l), f(l.pre_o), f(l.pre_m), f(l.pre_l),
                     reinterpret_cast<int32_t*>(ws + l.entry_at), reinterpret_cast<int32_t*>(ws + l.group_work),
                     reinterpret_cast<int32_t*>(ws + l.group_vec), splits, sms};
-  static bool pre_done[64] = {};
+  static bool pre_done[2][64] = {};
   if (groups.num_groups > 0) {
-    CUtensorMap kmap, vmap;
-    if (!make_tmap_kv(&kmap, k_cache, nkv, slots) || !make_tmap_kv(&vmap, v_cache, nkv, slots)) return NE_ERR_CUDA;
-    if (!allow_smem(prefix_kernel, PRE_SMEM, pre_done)) return NE_ERR_CUDA;
-    if (launch_kernel(prefix_kernel, dim3(sms), dim3(PRE_THREADS), PRE_SMEM, stream, kmap, vmap, q, rows, groups, nh,
-                      nkv, slots, parts, status) != cudaSuccess)
+    CUtensorMap kmap{}, vmap{};
+    if (!kv_int8 && (!make_tmap_kv(&kmap, k_cache, nkv, slots) || !make_tmap_kv(&vmap, v_cache, nkv, slots)))
+      return NE_ERR_CUDA;
+    auto kernel = kv_int8 ? prefix_kernel<true> : prefix_kernel<false>;
+    if (!allow_smem(kernel, PRE_SMEM, pre_done[kv_int8 ? 1 : 0])) return NE_ERR_CUDA;
+    if (launch_kernel(kernel, dim3(sms), dim3(pre_threads(kv_int8 != 0)), PRE_SMEM, stream, kmap, vmap,
+                      static_cast<const int8_t*>(k_cache), static_cast<const int8_t*>(v_cache), k_scale, v_scale, q, rows,
+                      groups, nh, nkv, slots, parts, status) != cudaSuccess)
       return NE_ERR_CUDA;
   }
   // one query tile of up to 16 vectors: eight warps where that leaves at most a CTA an SM, two where
