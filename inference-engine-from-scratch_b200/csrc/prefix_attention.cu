@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(32 * NW * NT, NT == 2 ? 2 : NW == 8 ? 1 : NW =
 
 // ---------------------------------------------------------------- prefixes: the tensor-core kernel
 // two softmax warpgroups; a load warp, two MMA warps, one idle; for an int8 pool four warps that load and
-// convert (which then run with 88 registers and leave the softmax 168: 512 x 128 at launch)
+// convert (128 registers a thread then; other splits of the registers were measured and are slower)
 constexpr int pre_threads(bool int8) { return int8 ? 512 : 384; }
 constexpr int SLOT_BYTES = TILE * D * 2;   // one K or V tile: two halves of 64 dimensions, rows of 128 B
 constexpr int RING = 4;
@@ -834,10 +834,6 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
   Walk walk(&plan, groups, nkv, G, per);
   Segment sg;
 
-  if (INT8) {
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  }
   if (warp < 8) {
     // ------------------------------------------------------------ softmax of query tile s, a row per thread
     const int s = warp >> 2, row = tid & 127;
@@ -1160,38 +1156,42 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
     while (ok && walk.next(sg)) {
       const int blocks = plan.blocks[sg.group];
       const int32_t* table = table_of(rows, plan.member[plan.group_first[sg.group]]);
+      int next[8];  // the next tile's block ids, loaded a tile ahead
+      auto look = [&](int t) {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) next[b] = t < sg.t1 && t * 8 + b < blocks ? table[t * 8 + b] : -1;
+      };
+      look(sg.t0);
       for (int t = sg.t0; ok && t < sg.t1; ++t, ++tile) {
         const uint32_t load = 2 * tile + is_v;
         const int slot = load % RING;
-        uint32_t mask = 0;
+        uint32_t mask = 0, bad = 0;
         uint4 x[16];
-        float scale[4];
+        long long own = -1;  // the block of keys 2 t64 and 2 t64 + 1, whose scales this thread brings
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
-          const int kb = t * 8 + b;
-          long long id = kb < blocks ? table[kb] : -1;
-          if (id < 0 || (id + 1) * 16 > num_cache_slots - 1) {
-            if (kb < blocks && t64 == 0) report(status, NE_DEV_BAD_SLOT);
-            id = -1;
-          }
-          mask |= (id >= 0 ? 1u : 0u) << b;
+          const long long id = next[b];
+          const bool in = id >= 0 && (id + 1) * 16 <= num_cache_slots - 1;
+          mask |= (in ? 1u : 0u) << b;
+          bad |= !in && t * 8 + b < blocks;
+          const long long at = ((in ? id * 16 : 0) + (t64 >> 3)) * nkv + sg.h;
 #pragma unroll
           for (int i = 2 * b; i < 2 * b + 2; ++i) {
             x[i] = make_uint4(0, 0, 0, 0);
-            if (id >= 0)
-              x[i] = *reinterpret_cast<const uint4*>(
-                  pool + ((id * 16 + 8 * (i & 1) + (t64 >> 3)) * nkv + sg.h) * (long long)D + 16 * ch);
+            if (in) x[i] = *reinterpret_cast<const uint4*>(pool + (at + 8 * (i & 1) * nkv) * D + 16 * ch);
           }
-          // the scales of keys 2 t64 and 2 t64 + 1
-          if (is_v && t64 >> 3 == b) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const long long at = (id * 16 + ((2 * t64 + i) & 15)) * nkv + sg.h;
-              scale[i] = id >= 0 ? __bfloat162float(ks[at]) * SCALE_LOG2 : 0.f;
-              scale[2 + i] = id >= 0 ? __bfloat162float(vs[at]) : 0.f;
-            }
-          }
+          if (in && t64 >> 3 == b) own = id;
         }
+        __nv_bfloat16 scale[4] = {};
+        if (is_v && own >= 0) {
+          const long long key = (own * 16 + (2 * t64 & 15)) * nkv + sg.h;
+          scale[0] = ks[key];
+          scale[1] = ks[key + nkv];
+          scale[2] = vs[key];
+          scale[3] = vs[key + nkv];
+        }
+        look(t + 1);
+        if (bad && t64 == 0) report(status, NE_DEV_BAD_SLOT);
         if (load >= RING) {
           ok = mbar_wait(&sh.empty[slot], (load / RING - 1) & 1u, &sh.abort_flag, status);
           ok = __all_sync(ALL, ok);
@@ -1213,8 +1213,10 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
           *reinterpret_cast<uint4*>(row + (((2 * ch + 1 & 7) ^ (key & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
         if (is_v) {
-          *reinterpret_cast<float2*>(&sh.scale[slot >> 1][0][2 * t64]) = make_float2(scale[0], scale[1]);
-          *reinterpret_cast<float2*>(&sh.scale[slot >> 1][1][2 * t64]) = make_float2(scale[2], scale[3]);
+          *reinterpret_cast<float2*>(&sh.scale[slot >> 1][0][2 * t64]) =
+              make_float2(__bfloat162float(scale[0]) * SCALE_LOG2, __bfloat162float(scale[1]) * SCALE_LOG2);
+          *reinterpret_cast<float2*>(&sh.scale[slot >> 1][1][2 * t64]) =
+              make_float2(__bfloat162float(scale[2]), __bfloat162float(scale[3]));
         }
         if (t64 == 0) sh.valid[slot] = mask;
         fence_proxy_async_smem();
