@@ -523,6 +523,16 @@ NE_API int ne_prefix_attention(const void* q, void* out, const void* k_cache, co
                                void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /*
+ * Let the model's steps use ne_prefix_attention in place of ne_paged_attention: forwards of up to 32
+ * query vectors per entry and KV head (speculative steps, single tokens) whose bounds fit the
+ * workspace; longer ones (prefills) keep the ordinary attention. The arrays are read by every such
+ * forward: entry_group [at least the forward's num_seqs] names the batch entries' groups, so a captured
+ * step follows their contents. groups NULL (or num_groups 0): off.
+ */
+NE_API int ne_model_set_prefix_groups(ne_model* model, const ne_prefix_groups* groups, void* workspace,
+                                      size_t workspace_bytes);
+
+/*
  * One draw per row of logits [rows, vocab] (bf16, or fp32 with ``logits_fp32``; rows ``row_stride``
  * elements apart) from given random numbers. With w_i = exp((x_i - max x) / temperature), the kept
  * tokens are the first n of the descending order (equal logits: lowest id first), n the least of

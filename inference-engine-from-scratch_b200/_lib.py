@@ -74,6 +74,7 @@ EXPORTS = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
          c_longlong, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
+    "ne_model_set_prefix_groups": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t]),
     "ne_sample_logits": (
         c_int,
         [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -46,6 +46,13 @@ int launch_attention_tc(const __nv_bfloat16* q, __nv_bfloat16* out, const void* 
                         const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8, const ne_rows& rows,
                         int num_heads, int num_kv_heads, long long num_cache_slots, const AttnSplit& sp, int* status,
                         cudaStream_t stream, const KvShadow& shadow = KvShadow{});
+// Attention over prompt prefixes that groups of entries share (prefix_attention.cu); NE_ERR_WORKSPACE when
+// ``ws`` (256-byte aligned) is too small for the launch's bounds.
+int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const void* k_cache, const void* v_cache,
+                            const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8,
+                            const ne_rows& rows, ne_prefix_groups groups, int num_heads, int num_kv_heads,
+                            long long num_cache_slots, uint8_t* ws, size_t ws_bytes, int* status,
+                            cudaStream_t stream);
 // Fill copies [first, first + num_blocks) from logical blocks 0.. of table row ``table`` (one layer),
 // then (once every layer is filled) map or unmap those pool blocks.
 int launch_kv_shadow_fill(const int32_t* table, int num_blocks, int first, const void* k_cache, const void* v_cache,

@@ -45,6 +45,10 @@ struct ne_model {
   __nv_bfloat16* kv_shadow = nullptr;
   int32_t* kv_shadow_map = nullptr;
   int kv_shadow_blocks = 0;
+  // shared-prefix attention of small steps: the groups of the batch entries (num_groups 0: off)
+  ne_prefix_groups prefix{};
+  uint8_t* prefix_ws = nullptr;
+  size_t prefix_ws_bytes = 0;
   // peer exchange (steps of up to link.max_rows rows): own region, peers' regions mapped here
   void* tp_region = nullptr;
   size_t tp_region_bytes = 0;
@@ -627,6 +631,24 @@ int ne_kv_shadow_clear(ne_model* m, const ne_batch_state* st, int src_slot, int 
                                   as_stream(stream));
 }
 
+int ne_model_set_prefix_groups(ne_model* m, const ne_prefix_groups* groups, void* workspace, size_t bytes) {
+  if (!m) return NE_ERR_INVALID;
+  if (!groups || groups->num_groups == 0) {
+    m->prefix = ne_prefix_groups{};
+    m->prefix_ws = nullptr;
+    m->prefix_ws_bytes = 0;
+    return NE_OK;
+  }
+  if (groups->num_groups < 0 || groups->num_groups > 1024 || groups->max_prefix_blocks < 1 || !groups->entry_group ||
+      !groups->prefix_blocks || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return NE_ERR_INVALID;
+  if (m->cfg.num_heads / m->cfg.num_kv_heads > 32) return NE_ERR_UNSUPPORTED;
+  m->prefix = *groups;
+  m->prefix_ws = static_cast<uint8_t*>(workspace);
+  m->prefix_ws_bytes = bytes;
+  return NE_OK;
+}
+
 int ne_model_tp_exchange_create(ne_model* m, int max_rows, void* ipc_handle) {
   if (!m || !ipc_handle || m->tp_world < 2 || m->tp_region || max_rows < 1 || max_rows > (1 << 16))
     return NE_ERR_INVALID;
@@ -677,7 +699,7 @@ int ne_forward(ne_model* m, const ne_rows* rows, int lm_mode, void* logits, int3
   if (lm_mode == NE_LM_LOGITS && !logits) return NE_ERR_INVALID;
   const bool tp = m->tp_world > 1;
   if (tp && lm_mode == NE_LM_LOGITS) return NE_ERR_UNSUPPORTED;  // logits are split over the ranks
-  if (use_step_kernel(m, rows, lm_mode)) return step_forward(m, rows, argmax_out, as_stream(stream));
+  if (m->prefix.num_groups == 0 && use_step_kernel(m, rows, lm_mode)) return step_forward(m, rows, argmax_out, as_stream(stream));
   // a split model exchanges partial rows through peer memory when they fit the exchange slots
   // (every rank takes the same branch: R and lm_max are the same host values on all ranks)
   const bool px = tp && m->link.world > 0 && R <= m->link.max_rows && rows->lm_max <= m->link.max_rows;
@@ -702,6 +724,11 @@ int ne_forward(ne_model* m, const ne_rows* rows, int lm_mode, void* logits, int3
                                                m->num_sms, m->attn_scratch_bytes);
   const ne::AttnSplit attn = ne::attention_split_view(m->attn_scratch, (long long)rows->num_seqs * c.num_kv_heads,
                                                       splits, max_vec);
+  // steps of up to two query tiles an entry read the prefixes that their entries share once
+  const bool shared = m->prefix.num_groups > 0 && max_vec <= 32 &&
+                      ne_prefix_attention_workspace_bytes(R, rows->num_seqs, m->prefix.num_groups, c.num_heads,
+                                                          c.num_kv_heads, std::max(1, rows->max_q_len),
+                                                          rows->max_context) <= m->prefix_ws_bytes;
   // rows the RMSNorm loads before reading the device row count: a speculative step's expected
   // rows plus a quarter (the bucket's bound is far above them: loading every row of it cost config
   // 4, 1,280 rows for ~500, 7.53 -> 7.95 ms per step)
@@ -741,7 +768,15 @@ int ne_forward(ne_model* m, const ne_rows* rows, int lm_mode, void* logits, int3
     rc = note(m, NE_K_GEMM_QKV, run_gemm(m, &m->tm_qkv[l], fuse ? &m->tm_h : &m->tm_x, R, rows->num_rows, qs + 2 * kvs, H,
                                          e, s, w.w_qkv_scale, fuse ? w.ln_in : nullptr), s);
     if (rc) return rc;
-    rc = note(m, NE_K_ATTENTION,
+    if (shared)
+      rc = note(m, NE_K_ATTENTION,
+                ne::launch_prefix_attention(m->q, m->attn, w.k_cache, w.v_cache,
+                                            static_cast<const __nv_bfloat16*>(w.k_scale),
+                                            static_cast<const __nv_bfloat16*>(w.v_scale), c.kv_int8, *rows, m->prefix,
+                                            c.num_heads, c.num_kv_heads, c.num_cache_slots, m->prefix_ws,
+                                            m->prefix_ws_bytes, m->status, s), s);
+    else
+      rc = note(m, NE_K_ATTENTION,
               ne::launch_attention_tc(m->q, m->attn, w.k_cache, w.v_cache,
                                       static_cast<const __nv_bfloat16*>(w.k_scale),
                                       static_cast<const __nv_bfloat16*>(w.v_scale), c.kv_int8, *rows, c.num_heads,

@@ -1280,6 +1280,10 @@ bool allow_smem(K kernel, size_t bytes, bool (&done)[64]) {
   return done[dev];
 }
 
+bool heads_ok(int nh, int nkv) { return nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= MAX_GROUP; }
+
+}  // namespace
+
 int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const void* k_cache, const void* v_cache,
                             const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8,
                             const ne_rows& rows, ne_prefix_groups groups, int nh, int nkv, long long slots,
@@ -1347,10 +1351,6 @@ int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const vo
              ? NE_OK
              : NE_ERR_CUDA;
 }
-
-bool heads_ok(int nh, int nkv) { return nkv > 0 && nh > 0 && nh % nkv == 0 && nh / nkv <= MAX_GROUP; }
-
-}  // namespace
 
 }  // namespace ne
 

@@ -101,8 +101,11 @@ class B200SpeculativeEngine:
         sampling: bool = False,
         draft_model: B200Model | None = None,
         draft_num_blocks: int | None = None,
+        shared_prefix_attention: bool = False,
     ) -> None:
-        """``draft_model``: drafts come from this smaller model of the same family
+        """``shared_prefix_attention``: steps read the blocks that their sequences share (``add_prefix``,
+        ``fork``) once for all of them (ne_prefix_attention) instead of once per sequence; the same
+        results up to rounding. ``draft_model``: drafts come from this smaller model of the same family
         (DraftModelProposer, engine/speculative/proposers.py:63-106; greedy requests) instead of
         n-gram lookup; it keeps its own batch state and KV pool (``draft_num_blocks`` blocks)."""
         self.lib = _lib.load()
@@ -166,11 +169,26 @@ class B200SpeculativeEngine:
                 self._region_bytes = self._region_rows * row_bytes
                 self._draft_regions = torch.empty(k * self._region_bytes, dtype=torch.uint8, device=model.device)
                 self._draft_stats = torch.empty(k * self._region_rows * 32, dtype=torch.uint8, device=model.device)
+        # the batch entries' prefix groups, on the device (and two host copies, as the slot list's)
+        self._groups_dev = self._groups_ws = None
+        if shared_prefix_attention:
+            if draft_model is not None:
+                raise ValueError("draft-model drafts serve requests without shared prefixes")
+            self._groups_dev = torch.zeros((2, max_seqs), dtype=torch.int32, device=model.device)
+            self._groups_hosts = [torch.zeros((2, max_seqs), dtype=torch.int32).pin_memory() for _ in range(2)]
+            cfg = model.cfg
+            need = max(int(self.lib.ne_prefix_attention_workspace_bytes(
+                b * (k + 1), b, max_seqs, cfg.num_attention_heads, cfg.num_key_value_heads, k + 1,
+                self.state.history_stride)) for b in self.buckets)
+            if need == 0 or (k + 1) * (cfg.num_attention_heads // cfg.num_key_value_heads) > 32:
+                raise ValueError("shared-prefix attention serves steps of up to 32 query vectors per KV head")
+            self._groups_ws = torch.empty(need, dtype=torch.uint8, device=model.device)
         self._uncached: dict[int, int] = {}       # slot -> prompt tokens still to prefill
         self._prefixes: dict[int, list] = {}      # holder slot -> [tokens, shared blocks, users, copies]
         self._prefix_of: dict[int, int] = {}      # slot -> holder slot of its shared prefix
         self._shared_count: dict[int, int] = {}   # slot -> blocks it shares with its prefix holder
         self._fork_of: dict[int, int] = {}        # forked slot -> the slot whose blocks it shares
+        self._fork_blocks: dict[int, int] = {}    # forked slot -> how many (shared-prefix attention)
         self.proposed_total = 0
         self.accepted_total = 0
         self.h2d_bytes = 0  # host->device bytes copied for requests and steps
@@ -311,6 +329,10 @@ class B200SpeculativeEngine:
             self.state.free_slots = slots + self.state.free_slots  # (they hold nothing)
             raise
         self.model.copy_blocks(src, dst)
+        if self._groups_dev is not None and n:
+            shared = int(self.state.num_shared_blocks[slots[0]].item())
+            self._fork_blocks.update((s, shared) for s in slots)
+        self._dev_slots_key = None  # (the same slots may now hold other sequences)
         for s in slots:
             self._uncached[s] = 1
             self._fork_of[s] = slot
@@ -338,6 +360,47 @@ class B200SpeculativeEngine:
             self.draft_model.copy_blocks(dsrc, ddst, dcount)
         return int(count.item())
 
+    def _prefix_group(self, slot: int) -> tuple[int, int]:
+        """(the slot whose first blocks ``slot`` shares, how many): its prefix's holder, or the source
+        its forks go back to."""
+        holder = self._prefix_of.get(slot)
+        if holder is not None:
+            return holder, self._shared_count[slot]
+        blocks = 1 << 30
+        while slot in self._fork_of:
+            blocks = min(blocks, self._fork_blocks[slot])
+            slot = self._fork_of[slot]
+        return slot, blocks
+
+    def _fill_groups(self, slots: list[int], host: torch.Tensor) -> None:
+        """Entry groups and prefix lengths of a batch: entries with the same root, two at least, share as
+        many blocks as the one among them that shares the fewest."""
+        members: dict[int, list[int]] = {}
+        shared: dict[int, int] = {}
+        for i, s in enumerate(slots):
+            root, blocks = self._prefix_group(s)
+            members.setdefault(root, []).append(i)
+            shared[root] = min(shared.get(root, 1 << 30), blocks)
+        entry_group, prefix_blocks = [-1] * self.max_seqs, [0] * self.max_seqs
+        g = 0
+        for root, entries in members.items():
+            if len(entries) > 1 and 0 < shared[root] < 1 << 30:
+                prefix_blocks[g] = shared[root]
+                for i in entries:
+                    entry_group[i] = g
+                g += 1
+        host.copy_(torch.tensor([entry_group, prefix_blocks], dtype=torch.int32))
+
+    def _bind_groups(self) -> None:
+        groups = None
+        if self._groups_dev is not None:
+            groups = _lib.PrefixGroups(num_groups=self.max_seqs, max_prefix_blocks=self.state.block_table_stride,
+                                       entry_group=self._groups_dev[0].data_ptr(),
+                                       prefix_blocks=self._groups_dev[1].data_ptr())
+        _lib.check(self.lib.ne_model_set_prefix_groups(
+            self.model.handle, None if groups is None else ctypes.byref(groups), _lib.ptr(self._groups_ws),
+            0 if self._groups_ws is None else self._groups_ws.numel()), "ne_model_set_prefix_groups")
+
     def release(self, slots: list[int]) -> None:
         for s, source in self._fork_of.items():
             if source in slots and s not in slots:
@@ -349,6 +412,7 @@ class B200SpeculativeEngine:
             self._uncached.pop(s, None)
             self._shared_count.pop(s, None)
             self._fork_of.pop(s, None)
+            self._fork_blocks.pop(s, None)
             holder = self._prefix_of.pop(s, None)
             if holder is not None:
                 self._prefixes[holder][2] -= 1
@@ -366,6 +430,10 @@ class B200SpeculativeEngine:
         self._slots_dev[:bucket].copy_(h[:bucket], non_blocking=True)
         self._dev_slots_key = key
         self.h2d_bytes += 4 * bucket
+        if self._groups_dev is not None:
+            self._fill_groups(slots, self._groups_hosts[host])
+            self._groups_dev.copy_(self._groups_hosts[host], non_blocking=True)
+            self.h2d_bytes += 4 * self._groups_dev.numel()
 
     def _collect(self, slots: list[int], outs: _Outputs | None = None) -> StepResult:
         outs = outs or self.outputs
@@ -419,6 +487,7 @@ class B200SpeculativeEngine:
     def _prefill_call(self, slots: list[int], rows: int, chunk: int) -> StepResult:
         self._set_slots(slots, len(slots))
         self._bind_sampler()
+        self._bind_groups()
         _lib.check(self.lib.ne_prefill(self.model.handle, self.state.ref, self._slots_dev.data_ptr(), len(slots),
                                        max(rows, 1), self.k, chunk, ctypes.byref(self.outputs.struct),
                                        _lib.stream_handle()), "ne_prefill")
@@ -439,6 +508,7 @@ class B200SpeculativeEngine:
     # ------------------------------------------------------------------ speculative step
     def _launch_step(self, bucket: int, buf: int = 0) -> None:
         self._bind_sampler()
+        self._bind_groups()
         if self.draft_state is None:
             _lib.check(self.lib.ne_spec_step(self.model.handle, self.state.ref, self._slots_dev.data_ptr(), bucket,
                                              self.k, self.max_ngram, ctypes.byref(self._outs[buf].struct),

@@ -1,0 +1,148 @@
+"""The operators for many samples of one prompt in the engine, together: shared prefixes and forks
+whose steps read the shared blocks once (``shared_prefix_attention``), drawn with ``ops.sample_logits``
+and moved by compaction."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from tests.conftest import submodule
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def make(pkg, cuda_device):
+    submodule("build").build()
+    weights = pkg.make_weights(pkg.SMALL_TEST, seed=0)
+    models = {}
+
+    def engine(kv_int8=False, shared=True, max_seqs=8, **kw):
+        if kv_int8 not in models:
+            models[kv_int8] = submodule("model").B200Model(
+                pkg.SMALL_TEST, weights, num_slots=192 * 16, device=cuda_device, max_positions=640, max_rows=512,
+                max_seqs=16, kv_int8=kv_int8)
+        return submodule("engine").B200SpeculativeEngine(models[kv_int8], k=4, max_ngram=3, max_seqs=max_seqs,
+                                                         max_model_len=512, num_blocks=192, sampling=True,
+                                                         shared_prefix_attention=shared, **kw)
+
+    return engine
+
+
+def prompts_with_prefix(pkg, length, n):
+    v = pkg.SMALL_TEST.vocab_size
+    prefix = pkg.make_prompt(v, length, 3, False)
+    return [prefix + pkg.make_prompt(v, 5 + 3 * i, 50 + i, i % 2 == 0) for i in range(n)]
+
+
+@pytest.mark.parametrize("kv_int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("graphs", [True, False], ids=["graphs", "eager"])
+def test_shared_prefix_requests_take_the_same_tokens(pkg, make, kv_int8, graphs) -> None:
+    """Greedy requests on one prefix (more than fit at once, so slots change hands under captured steps)."""
+    prompts = prompts_with_prefix(pkg, 200, 11)
+    want = make(kv_int8, shared=False).generate(prompts, 20, shared_prefix=200)
+    eng = make(kv_int8, cuda_graphs=graphs)
+    assert eng.generate(prompts, 20, shared_prefix=200) == want
+    assert eng.state.num_free_blocks() == 192
+    # and the same engine without any sharing
+    assert eng.generate(prompts[:5], 12) == make(kv_int8, shared=False).generate(prompts[:5], 12)
+
+
+def test_two_prefixes_forks_and_loners_in_one_batch(pkg, make) -> None:
+    a, b = prompts_with_prefix(pkg, 150, 2), [p[70:] for p in prompts_with_prefix(pkg, 150, 4)[2:]]
+    lone = pkg.make_prompt(pkg.SMALL_TEST.vocab_size, 40, 9, False)
+    outs = {}
+    for shared in (False, True):
+        eng = make(shared=shared)
+        pa, pb = eng.add_prefix(a[0][:150]), eng.add_prefix(b[0][:80])
+        slots = eng.add_requests(a, [24, 24], ignore_eos=True, prefix=pa)
+        slots += eng.add_requests(b, [24, 24], ignore_eos=True, prefix=pb)
+        slots.append(eng.add_request(lone, 24, ignore_eos=True))
+        res = eng.prefill(slots)
+        out = {s: list(res.tokens[s]) for s in slots}
+        for _ in range(2):
+            for s, t in eng.step(slots).tokens.items():
+                out[s] += t
+        fork, = eng.fork(slots[-1])
+        slots.append(fork)
+        out[fork] = list(out[slots[-2]])
+        eng.compact()
+        live = list(slots)
+        while live:
+            res = eng.step(live)
+            for s in list(live):
+                out[s] += res.tokens[s]
+                if res.finish[s] is not None:
+                    live.remove(s)
+        outs[shared] = [out[s] for s in slots]
+        eng.release(slots)
+        eng.drop_prefix(pa)
+        eng.drop_prefix(pb)
+        assert eng.state.num_free_blocks() == 192
+    assert outs[True] == outs[False]
+    assert outs[True][-1] == outs[True][-2]
+
+
+def test_a_fork_in_a_reused_slot_gets_its_own_group(pkg, make) -> None:
+    """The step's slot list stays the same while the fork in it is another one: the groups follow."""
+    eng = make(max_seqs=2)
+    prompt = prompts_with_prefix(pkg, 100, 1)[0]
+    want = make(shared=False).generate([prompt], 60)[0]
+    s = eng.add_request(prompt, 60, ignore_eos=True)
+    out = list(eng.prefill([s]).tokens[s])
+    for _ in range(3):
+        fork, = eng.fork(s)
+        theirs = list(out)
+        for _ in range(4):
+            res = eng.step(sorted([s, fork]))
+            out += res.tokens[s]
+            theirs += res.tokens[fork]
+        assert theirs == out
+        eng.release([fork])
+    while len(out) < 60:
+        out += eng.step([s]).tokens[s]
+    assert out == want
+
+
+def test_fork_step_and_sample_by_hand(pkg, make, cuda_device) -> None:
+    """A user's own loop: prefill, fork, one step, and next tokens drawn from the step's logits with
+    top-k, top-p and min-p; the draw equals the definition on those logits."""
+    from tests.test_gpu_sample_logits import check
+
+    ops = submodule("ops")
+    eng = make()
+    prompt = prompts_with_prefix(pkg, 120, 1)[0]
+    s = eng.add_request(prompt, 40, ignore_eos=True, temperature=0.9, top_p=0.95, seed=1)
+    eng.prefill([s])
+    slots = [s] + eng.fork(s, 5, at=len(prompt), seeds=[2, 3, 4, 5, 6])
+    eng.step(slots)
+    rows = 6
+    logits = eng.sampled_logits(rows)
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    check(ops, logits, [(0.8, 20, 0.9, 0.01)] * rows, u)
+    eng.release(slots)
+
+
+def test_model_entry_refuses_bad_arguments(pkg, make, cuda_device) -> None:
+    _lib = submodule("_lib")
+    eng = make()
+    lib, handle = eng.lib, eng.model.handle
+    some = torch.zeros(256, dtype=torch.int32, device=cuda_device)
+    ok = dict(num_groups=1, max_prefix_blocks=4, entry_group=some.data_ptr(), prefix_blocks=some.data_ptr())
+    call = lambda ws=some.data_ptr(), **kw: lib.ne_model_set_prefix_groups(  # noqa: E731
+        handle, ctypes.byref(_lib.PrefixGroups(**{**ok, **kw})), ws, 1024)
+    assert lib.ne_model_set_prefix_groups(None, None, None, 0) == 1
+    for bad in (dict(num_groups=-1), dict(num_groups=1025), dict(max_prefix_blocks=0), dict(entry_group=None),
+                dict(prefix_blocks=None), dict(ws=None), dict(ws=some.data_ptr() + 4)):
+        assert call(**bad) == 1
+    assert call() == 0  # (a workspace too small for a step: its attention stays the ordinary one)
+    prompt = prompts_with_prefix(pkg, 60, 1)[0]
+    assert eng.generate([prompt], 8) == make(shared=False).generate([prompt], 8)
+    assert lib.ne_model_set_prefix_groups(handle, None, None, 0) == 0
+    with pytest.raises(ValueError):
+        make(draft_model=submodule("model").B200Model(
+            pkg.SMALL_TEST, pkg.make_weights(pkg.SMALL_TEST, seed=1), num_slots=32 * 16, device=cuda_device,
+            max_positions=640, max_rows=512, max_seqs=16))
