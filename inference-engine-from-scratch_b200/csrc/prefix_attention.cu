@@ -1112,10 +1112,7 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
     while (ok && walk.next(sg)) {
       const int tiles = sg.t1 - sg.t0;
       const bool both = sg.nv > TILE;
-      auto release = [&](uint32_t at) {
-        tc_commit(&sh.empty[(base + at) % RING]);
-        if (!both) tc_commit(&sh.empty[(base + at) % RING]);  // (for the query tile that is not there)
-      };
+      auto release = [&](uint32_t at) { tc_commit(&sh.empty[(base + at) % RING]); };
       if (both || s == 0) {
         begun = false;
         if (!wait(&sh.q_ready[s], q_phase++) || !full(0)) break;
@@ -1141,11 +1138,17 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
           }
         }
         tiles_before += tiles;
+      } else {
+        // no second query tile: its thread still takes part in every slot's turn. (Left to run ahead, it
+        // would wait for a slot two turns on, whose parity the turn before it already shows.)
+        for (int at = 0; at < 2 * tiles; ++at) {
+          if (!full(at)) break;
+          mbar_arrive(&sh.empty[(base + at) % RING]);
+        }
       }
       base += 2 * tiles;
     }
-  }
-  else if (INT8 && warp >= 12) {
+  } else if (INT8 && warp >= 12) {
     // ------------------------------------------------------------ int8 loads: two warps for K, two for V
     // A tile is 1024 pieces of 16 integers: thread t takes pieces t + 64 i, all loads issued before the
     // slot is free, and writes each as bf16 (exact) where a tensor load would have put it.

@@ -145,6 +145,20 @@ CASES = {
 }
 
 
+def _mixed(groups, blocks):
+    """Groups of one query tile and of two in turn, so that a CTA's share of the work holds both."""
+    q_lens, group = [], []
+    for g in range(groups):
+        for _ in range(1 if g % 2 else 10):
+            q_lens.append(2 if g % 2 else 5)
+            group.append(g)
+    return (32, 8, q_lens, [16 * (blocks - g % 7) for g in range(groups)], group, [i % 23 for i in range(len(q_lens))])
+
+
+CASES["one_and_two_tiles_in_turn"] = _mixed(40, 70)
+CASES["one_and_two_tiles_short"] = _mixed(60, 20)
+
+
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
 @pytest.mark.parametrize("name", list(CASES))
 def test_matches_64_bits(ops, name, int8) -> None:
