@@ -230,6 +230,8 @@ class B200SpeculativeEngine:
             if len(prompt) == 0 or len(prompt) + new > self.state.max_model_len:
                 raise ValueError(f"prompt of {len(prompt)} + {new} new tokens exceeds max_model_len")
         slots = [self.state.acquire() for _ in range(n)]
+        if self._groups_dev is not None:
+            self._dev_slots_key = None  # (slots listed before may now share other blocks, or none)
         self.state.load_many(slots, prompts, list(max_new_tokens), ignore_eos=[ignore_eos] * n,
                              temperature=[temperature] * n, top_p=[top_p] * n, seed=seeds, draws=draws)
         per_request = 5 * 4 + 4 + 4 + 8 + 8

@@ -107,6 +107,33 @@ def test_a_fork_in_a_reused_slot_gets_its_own_group(pkg, make) -> None:
     assert out == want
 
 
+def test_requests_in_reused_slots_leave_the_old_group(pkg, make) -> None:
+    """Two requests on a prefix, then two without one in the same slots: the slot list stays the same."""
+    shared = prompts_with_prefix(pkg, 200, 2)
+    v = pkg.SMALL_TEST.vocab_size
+    lone = [pkg.make_prompt(v, 230, 70 + i, i == 0) for i in range(2)]
+    outs = {}
+    for on in (False, True):
+        eng = make(shared=on, max_seqs=3)
+        holder = eng.add_prefix(shared[0][:200])
+        outs[on] = []
+        for prompts, prefix in ((shared, holder), (lone, None), (shared, holder)):
+            slots = eng.add_requests(prompts, [20, 20], ignore_eos=True, prefix=prefix)
+            assert sorted(slots) == [1, 2]
+            res = eng.prefill(slots)
+            out = {s: list(res.tokens[s]) for s in slots}
+            live = list(slots)
+            while live:
+                res = eng.step(live)
+                for s in list(live):
+                    out[s] += res.tokens[s]
+                    if res.finish[s] is not None:
+                        live.remove(s)
+            outs[on].append([out[s] for s in slots])
+            eng.release([1, 2])
+    assert outs[True] == outs[False]
+
+
 def test_fork_step_and_sample_by_hand(pkg, make, cuda_device) -> None:
     """A user's own loop: prefill, fork, one step, and next tokens drawn from the step's logits with
     top-k, top-p and min-p; the draw equals the definition on those logits."""
