@@ -341,7 +341,8 @@ class B200SpeculativeEngine:
             if slot in self._prefix_of:  # the prefix's blocks are theirs as well
                 self._prefix_of[s] = self._prefix_of[slot]
                 self._prefixes[self._prefix_of[slot]][2] += 1
-                self._shared_count[s] = self._shared_count[slot]
+                # (a fork cut inside the prefix shares the full blocks before its last token)
+                self._shared_count[s] = min(self._shared_count[slot], (at - 1) // 16 if at else 1 << 30)
         return slots
 
     def trim(self, slots: list[int]) -> None:

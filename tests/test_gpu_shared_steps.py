@@ -134,6 +134,31 @@ def test_requests_in_reused_slots_leave_the_old_group(pkg, make) -> None:
     assert outs[True] == outs[False]
 
 
+@pytest.mark.parametrize("at", [1, 33, 48, 49, 160, 170])
+def test_a_fork_cut_inside_the_prefix(pkg, make, at) -> None:
+    """The fork shares fewer blocks than its source does: the group reads those only."""
+    prompt = prompts_with_prefix(pkg, 160, 1)[0] + pkg.make_prompt(pkg.SMALL_TEST.vocab_size, 12, 8, False)
+    outs = {}
+    for on in (False, True):
+        eng = make(shared=on)
+        holder = eng.add_prefix(prompt[:160])
+        s = eng.add_request(prompt, 16, ignore_eos=True, prefix=holder)
+        eng.prefill([s])
+        slots = [s] + eng.fork(s, 2, at=at)
+        out = {i: [] for i in slots}
+        for _ in range(4):
+            for i, t in eng.step(slots).tokens.items():
+                out[i] += t
+        outs[on] = [out[i] for i in slots]
+        eng.release(slots)
+        eng.drop_prefix(holder)
+        assert eng.state.num_free_blocks() == 192
+    assert outs[True] == outs[False]
+    want = make(shared=False).generate([prompt[:at]], 8)[0]
+    n = min(len(want), len(outs[True][1]))
+    assert n >= 4 and outs[True][1][:n] == want[:n] and outs[True][2] == outs[True][1]
+
+
 def test_fork_step_and_sample_by_hand(pkg, make, cuda_device) -> None:
     """A user's own loop: prefill, fork, one step, and next tokens drawn from the step's logits with
     top-k, top-p and min-p; the draw equals the definition on those logits."""
