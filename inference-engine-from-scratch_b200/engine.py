@@ -16,6 +16,7 @@ device->host (tokens, counts, finish reasons, proposed / accepted) in one copy.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass, field
 
@@ -180,8 +181,9 @@ class B200SpeculativeEngine:
             need = max(int(self.lib.ne_prefix_attention_workspace_bytes(
                 b * (k + 1), b, max_seqs, cfg.num_attention_heads, cfg.num_key_value_heads, k + 1,
                 self.state.history_stride)) for b in self.buckets)
-            if need == 0 or (k + 1) * (cfg.num_attention_heads // cfg.num_key_value_heads) > 32:
-                raise ValueError("shared-prefix attention serves steps of up to 32 query vectors per KV head")
+            if max_seqs > 1024 or need == 0 or (k + 1) * (cfg.num_attention_heads // cfg.num_key_value_heads) > 32:
+                raise ValueError("shared-prefix attention serves up to 1024 sequences and steps of up to 32 query "
+                                 "vectors per KV head")
             self._groups_ws = torch.empty(need, dtype=torch.uint8, device=model.device)
         self._uncached: dict[int, int] = {}       # slot -> prompt tokens still to prefill
         self._prefixes: dict[int, list] = {}      # holder slot -> [tokens, shared blocks, users, copies]
@@ -394,15 +396,23 @@ class B200SpeculativeEngine:
                 g += 1
         host.copy_(torch.tensor([entry_group, prefix_blocks], dtype=torch.int32))
 
-    def _bind_groups(self) -> None:
-        groups = None
-        if self._groups_dev is not None:
-            groups = _lib.PrefixGroups(num_groups=self.max_seqs, max_prefix_blocks=self.state.block_table_stride,
-                                       entry_group=self._groups_dev[0].data_ptr(),
-                                       prefix_blocks=self._groups_dev[1].data_ptr())
-        _lib.check(self.lib.ne_model_set_prefix_groups(
-            self.model.handle, None if groups is None else ctypes.byref(groups), _lib.ptr(self._groups_ws),
-            0 if self._groups_ws is None else self._groups_ws.numel()), "ne_model_set_prefix_groups")
+    @contextlib.contextmanager
+    def _bound_groups(self, entries: int):
+        """The model reads this engine's groups in the launches inside, and in no other user's. (One
+        entry shares with none, and keeps the one-sequence step.)"""
+        if self._groups_dev is None or entries < 2:
+            yield
+            return
+        groups = _lib.PrefixGroups(num_groups=self.max_seqs, max_prefix_blocks=self.state.block_table_stride,
+                                   entry_group=self._groups_dev[0].data_ptr(),
+                                   prefix_blocks=self._groups_dev[1].data_ptr())
+        _lib.check(self.lib.ne_model_set_prefix_groups(self.model.handle, ctypes.byref(groups),
+                                                       self._groups_ws.data_ptr(), self._groups_ws.numel()),
+                   "ne_model_set_prefix_groups")
+        try:
+            yield
+        finally:
+            self.lib.ne_model_set_prefix_groups(self.model.handle, None, None, 0)
 
     def release(self, slots: list[int]) -> None:
         for s, source in self._fork_of.items():
@@ -490,10 +500,10 @@ class B200SpeculativeEngine:
     def _prefill_call(self, slots: list[int], rows: int, chunk: int) -> StepResult:
         self._set_slots(slots, len(slots))
         self._bind_sampler()
-        self._bind_groups()
-        _lib.check(self.lib.ne_prefill(self.model.handle, self.state.ref, self._slots_dev.data_ptr(), len(slots),
-                                       max(rows, 1), self.k, chunk, ctypes.byref(self.outputs.struct),
-                                       _lib.stream_handle()), "ne_prefill")
+        with self._bound_groups(len(slots)):
+            _lib.check(self.lib.ne_prefill(self.model.handle, self.state.ref, self._slots_dev.data_ptr(), len(slots),
+                                           max(rows, 1), self.k, chunk, ctypes.byref(self.outputs.struct),
+                                           _lib.stream_handle()), "ne_prefill")
         if self.draft_state is not None:
             # the draft model prefills the same prompt tokens into its own cache (its own first
             # token is replaced by the target's at the next ne_draft_sync)
@@ -511,11 +521,11 @@ class B200SpeculativeEngine:
     # ------------------------------------------------------------------ speculative step
     def _launch_step(self, bucket: int, buf: int = 0) -> None:
         self._bind_sampler()
-        self._bind_groups()
         if self.draft_state is None:
-            _lib.check(self.lib.ne_spec_step(self.model.handle, self.state.ref, self._slots_dev.data_ptr(), bucket,
-                                             self.k, self.max_ngram, ctypes.byref(self._outs[buf].struct),
-                                             _lib.stream_handle()), "ne_spec_step")
+            with self._bound_groups(bucket):
+                _lib.check(self.lib.ne_spec_step(self.model.handle, self.state.ref, self._slots_dev.data_ptr(), bucket,
+                                                 self.k, self.max_ngram, ctypes.byref(self._outs[buf].struct),
+                                                 _lib.stream_handle()), "ne_spec_step")
             return
         # draft model: sync with the target, k greedy draft steps (the first catches up), verify
         stream, slots = _lib.stream_handle(), self._slots_dev.data_ptr()

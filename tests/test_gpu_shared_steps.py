@@ -178,6 +178,34 @@ def test_fork_step_and_sample_by_hand(pkg, make, cuda_device) -> None:
     eng.release(slots)
 
 
+@pytest.mark.parametrize("graphs", [True, False], ids=["graphs", "eager"])
+def test_the_model_keeps_no_groups_between_launches(pkg, make, graphs) -> None:
+    """The groups' arrays are the engine's: other users of the model, and later ones, never read them."""
+    class Recorder:
+        def __init__(self, lib):
+            self.lib, self.bound = lib, []
+
+        def __getattr__(self, name):
+            return getattr(self.lib, name)
+
+        def ne_model_set_prefix_groups(self, handle, groups, ws, size):
+            self.bound.append(groups is not None)
+            return self.lib.ne_model_set_prefix_groups(handle, groups, ws, size)
+
+    prompts = prompts_with_prefix(pkg, 200, 3)
+    eng = make(cuda_graphs=graphs)
+    eng.lib = recorder = Recorder(eng.lib)
+    eng.generate(prompts, 6, shared_prefix=200)
+    n = len(recorder.bound)
+    assert n and recorder.bound == [True, False] * (n // 2)
+    recorder.ne_prefill = lambda *args: 1
+    slots = eng.add_requests(prompts, [4] * 3)
+    with pytest.raises(Exception):
+        eng.prefill(slots)
+    assert recorder.bound[n:] == [True, False]
+    eng.release(slots)
+
+
 def test_model_entry_refuses_bad_arguments(pkg, make, cuda_device) -> None:
     _lib = submodule("_lib")
     eng = make()
