@@ -610,12 +610,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^t for two finite t up to 126 (below -126: 2^-126), on the FMA pipe beside the special-function one:
+// 2^t for two t up to 126 (0 below 2^-127, as the special-function one flushes), on the FMA pipe beside the special-function one:
 // t = n + f, n = rint(t) read off the low bits of t + 1.5 x 2^23, and 2^f on [-1/2, 1/2] by the cubic
 // whose largest relative error is least (7.5e-5; the weight is rounded to bf16, 2^-9, next).
 __device__ __forceinline__ void ex2_poly(uint64_t t2, float& a, float& b) {
   unpack2(t2, a, b);
-  t2 = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  t2 = pack2(fmaxf(a, -127.f), fmaxf(b, -127.f));
   constexpr float MAGIC = 12582912.f;
   constexpr float C0 = 0.99992806f, C1 = 0.69326097f, C2 = 0.24261113f, C3 = 0.05517165f;
   const uint64_t n2 = add2(t2, pack2(MAGIC, MAGIC));
@@ -626,8 +626,9 @@ __device__ __forceinline__ void ex2_poly(uint64_t t2, float& a, float& b) {
   float na, nb;
   unpack2(n2, na, nb);
   unpack2(y2, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
+  // (an exponent below the smallest leaves the integer negative)
+  a = __int_as_float(max(__float_as_int(a) + (__float_as_int(na) << 23), 0));
+  b = __int_as_float(max(__float_as_int(b) + (__float_as_int(nb) << 23), 0));
 }
 
 // A CTA's part of one item: vectors [v0, v0 + nv) of (group, head), key tiles [t0, t1).
@@ -778,12 +779,13 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
   }
   __syncthreads();
   if (warp == 0) {
-    int work = 0, vecs = 0, members = 0;
+    // (rows below 2^30 in all, whatever the entries say; work and vectors count only if they pass the test)
+    int work = 0, taken = 0, members = 0;
     for (int g0 = 0; g0 < ng; g0 += 32) {
       const int g = g0 + lane;
-      const int vec = g < ng ? plan.vec[g] * G : 0, count = g < ng ? plan.group_first[g] : 0;
-      const int w = vec ? nkv * head_work(vec, plan.blocks[g]) : 0;
-      int wi = w, vi = vec, mi = count;
+      const int mine = g < ng ? plan.vec[g] : 0, count = g < ng ? plan.group_first[g] : 0;
+      const int w = mine ? nkv * head_work(mine * G, plan.blocks[g]) : 0;
+      int wi = w, vi = mine, mi = count;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int a = __shfl_up_sync(ALL, wi, o), c = __shfl_up_sync(ALL, vi, o), d = __shfl_up_sync(ALL, mi, o);
@@ -795,22 +797,22 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
       }
       if (g < ng) {
         plan.work[g] = work + wi - w;
-        plan.vec[g] = vecs + vi - vec;
+        plan.vec[g] = (taken + vi - mine) * G;
         plan.group_first[g] = members + mi - count;
       }
       work += __shfl_sync(ALL, wi, 31);
-      vecs += __shfl_sync(ALL, vi, 31);
+      taken += __shfl_sync(ALL, vi, 31);
       members += __shfl_sync(ALL, mi, 31);
     }
     __syncwarp();
-    if (vecs > rows.max_rows * G) {  // entries that share rows: more parts than there is room for
+    if (taken > rows.max_rows) {  // entries that share rows: more parts than there is room for
       if (lane == 0) report(status, NE_DEV_BAD_SLOT);
       for (int g = lane; g < ng; g += 32) plan.work[g] = 0;
       work = 0;
     }
     if (lane == 0) {
       plan.work[ng] = work;
-      plan.vec[ng] = vecs;
+      plan.vec[ng] = taken * G;
       plan.members = members;
     }
     __syncwarp();
@@ -1040,7 +1042,7 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           id[x] = next[x];
-          if (id[x] >= 0 && (long long)(id[x] + 1) * 16 <= num_cache_slots - 1) mask |= 1u << x;
+          if (id[x] >= 0 && ((long long)id[x] + 1) * 16 <= num_cache_slots - 1) mask |= 1u << x;
           else if (t * 8 + x < blocks) report(status, NE_DEV_BAD_SLOT);
         }
         look(t + 1);
@@ -1241,9 +1243,9 @@ constexpr int JOIN_WARPS = 8;
 // their sums of weights, their values), the inputs before it.
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
     join_kernel(__nv_bfloat16* __restrict__ out, ne_rows rows, ne_prefix_groups groups, int nh, int nkv, Parts parts) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.y;
   const Entry e = entry_of(rows, groups, b, nullptr);
-  const int x = blockIdx.y * JOIN_WARPS + warp, blocks = e.group >= 0 ? groups.prefix_blocks[e.group] : 0;
+  const int x = blockIdx.x * JOIN_WARPS + warp, blocks = e.group >= 0 ? groups.prefix_blocks[e.group] : 0;
   pdl_prologue();
   if (x >= e.rows * nh) return;
   const int j = x / nh, head = x % nh, G = nh / nkv;
@@ -1349,7 +1351,7 @@ int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const vo
   }
   if (rc != NE_OK) return rc;
   const long long vectors = (long long)rows.max_q_len * nh;
-  return launch_kernel(join_kernel, dim3(rows.num_seqs, (unsigned)((vectors + JOIN_WARPS - 1) / JOIN_WARPS)),
+  return launch_kernel(join_kernel, dim3((unsigned)((vectors + JOIN_WARPS - 1) / JOIN_WARPS), rows.num_seqs),
                        dim3(32 * JOIN_WARPS), 0, stream, out, rows, groups, nh, nkv, parts) == cudaSuccess
              ? NE_OK
              : NE_ERR_CUDA;

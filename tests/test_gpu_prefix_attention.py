@@ -265,7 +265,7 @@ def test_rows_out_of_order_and_table_rows_by_index(ops) -> None:
     torch.testing.assert_close(got.float(), want[perm].float(), rtol=2 ** -6, atol=2 ** -6)
 
 
-@pytest.mark.parametrize("bad", [-1, 1 << 20])
+@pytest.mark.parametrize("bad", [-1, 1 << 20, (1 << 31) - 1, -(1 << 31)])
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
 def test_an_id_outside_the_pool_is_reported_and_left_out(ops, bad, int8) -> None:
     c = make_case(11, 16, 8, [3, 3], [160], [0, 0], [40, 50], int8=int8)
@@ -273,6 +273,39 @@ def test_an_id_outside_the_pool_is_reported_and_left_out(ops, bad, int8) -> None
     c["table"][1, 11] = bad  # inside entry 1's own blocks
     got, status = call(ops, c)
     assert int(status.item()) == BAD_SLOT
+    assert_close(got, c)
+
+
+def test_entries_that_share_rows_are_reported(ops) -> None:
+    """More rows of groups than there are rows: the prefixes are left out, nothing past the buffers is written."""
+    c = make_case(20, 16, 8, [4, 4, 4], [64], [0, 0, 0], [5, 6, 7])
+    c["q_start"].zero_()
+    for name in ("q", "positions"):
+        c[name] = c[name][:4].contiguous()
+    got, status = call(ops, c)
+    assert int(status.item()) == BAD_SLOT
+    assert bool(torch.isfinite(got).all())
+
+
+def test_a_bound_of_many_rows_an_entry(ops) -> None:
+    """A captured prefill's bound may be far above the rows of a replay."""
+    c = make_case(21, 16, 8, [3, 40], [160], [0, 0], [7, 30])
+    got, status = call(ops, c, max_q_len=1 << 16, max_context=1 << 17)
+    assert int(status.item()) == 0
+    assert_close(got, c)
+
+
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_a_large_value_at_a_key_of_no_weight_stays_out(ops, where) -> None:
+    """Weights below fp32's range are zero, not its least number: 3e38 times that would be seen."""
+    c = make_case(22, 16, 8, [5] * 4, [272], [0] * 4, [40, 30, 20, 35])
+    c["q"] = c["q"].abs()
+    entry, at = (0, 75) if where == "prefix" else (1, 280)
+    slot = int(c["table"][entry][at // BLOCK]) * BLOCK + at % BLOCK
+    c["k"][slot] = -60.0
+    c["v"][slot] = 3e38
+    got, status = call(ops, c)
+    assert int(status.item()) == 0
     assert_close(got, c)
 
 
