@@ -173,6 +173,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
+// (0 for 64 places and more, which C++ leaves open)
+__device__ __forceinline__ unsigned long long shift_right(unsigned long long v, int by) {
+  unsigned long long d;
+  asm("shr.u64 %0, %1, %2;" : "=l"(d) : "l"(v), "r"(by));
+  return d;
+}
+
 template <typename T>
 struct Row {
   const uint4* vecs;   // this CTA's slice: vector v holds tokens PER v .. of it, padded with -inf
@@ -180,28 +187,28 @@ struct Row {
   uint32_t top;        // the row's largest key
   bool inf;            // it alone has a weight
   bool careful;        // (a temperature so high that masked logits have to be told apart by their keys)
-  float least;         // a logit whose weight is 2^-60
-  float c1, c2;        // log2(e) / temperature = c1 + c2
-  float mp, me, ml;    // the largest logit times c1 (its product, and the rounding error of that) and c2
+  float least;         // a logit whose weight is 2^-59 or less
+  float scale, minus;  // 1, or what keeps differences and c1 in range; minus the largest logit times it
+  float c1, c2;        // log2(e) / (temperature x scale) = c1 + c2
   const uint2* pow2;
 
   // exp((x - m) / T) in steps of 2^-45: 2^t, t = (x - m) log2(e) / T = n / 64 + r, |r| <= 1/128, as the
   // table's 2^(n / 64) times the series of 2^r to the fourth power. On the FMA and integer pipes: the
-  // products x c and m c are taken with their rounding errors, and their difference with its own, so
-  // that t is off by less than 2^-30; the weight by about 2e-9 of itself, each logit's differently.
+  // difference and its product with c are taken with their rounding errors, so that t is off by less than
+  // 2^-30 whatever the largest logit; the weight by about 2e-9 of itself, each logit's differently.
   // (The same in fp64 took a pass over a row from 6 to 25 us.) A logit below ``least``, -inf or NaN
-  // weighs 2^-60, which is 0.
+  // weighs 2^-59 or less, which is 0.
   __device__ __forceinline__ void power2(float logit_a, float logit_b, unsigned long long& wa, unsigned long long& wb,
                                          int* band = nullptr, float* approx = nullptr) const {
     constexpr uint64_t MINUS = 0xBF800000BF800000ull;         // (-1, -1): a - b as fma(b, -1, a), one rounding
-    const uint64_t x = pair(fmaxf(logit_a, least), fmaxf(logit_b, least)), c = pair(c1, c1), m2 = pair(mp, mp);
-    const uint64_t p = mul2(x, c), e = fma2(x, c, mul2(p, MINUS));  // x c1 = p + e
-    const uint64_t s = fma2(m2, MINUS, p), z = fma2(p, MINUS, s);   // p - mp = s + err
-    const uint64_t err = fma2(add2(m2, z), MINUS, fma2(fma2(z, MINUS, s), MINUS, p));
-    const uint64_t low = add2(err, add2(fma2(pair(me, me), MINUS, e), fma2(x, pair(c2, c2), pair(-ml, -ml))));
-    constexpr float MAGIC = 196608.f;                         // 1.5 x 2^17: s rounded to 1 / 64
-    const uint64_t u = add2(s, pair(MAGIC, MAGIC));
-    const uint64_t r = add2(fma2(add2(u, pair(-MAGIC, -MAGIC)), MINUS, s), low);
+    const uint64_t x = pair(fmaxf(logit_a, least), fmaxf(logit_b, least)), c = pair(c1, c1), m2 = pair(minus, minus);
+    const uint64_t s = fma2(x, pair(scale, scale), m2), z = fma2(x, pair(-scale, -scale), s);  // x - m = s + err
+    const uint64_t err = add2(fma2(x, pair(scale, scale), fma2(s, MINUS, z)), fma2(z, MINUS, m2));
+    const uint64_t p = mul2(s, c), e = fma2(s, c, mul2(p, MINUS));  // s c1 = p + e
+    const uint64_t low = fma2(err, c, fma2(s, pair(c2, c2), e));
+    constexpr float MAGIC = 196608.f;                         // 1.5 x 2^17: p rounded to 1 / 64
+    const uint64_t u = add2(p, pair(MAGIC, MAGIC));
+    const uint64_t r = add2(fma2(add2(u, pair(-MAGIC, -MAGIC)), MINUS, p), low);
     uint64_t y = fma2(r, pair(0.009618129f, 0.009618129f), pair(0.05550411f, 0.05550411f));
     y = fma2(y, r, pair(0.24022651f, 0.24022651f));
     y = mul2(fma2(y, r, pair(0.69314718f, 0.69314718f)), r);  // 2^r - 1
@@ -211,8 +218,8 @@ struct Row {
     // (|y| < 0.0055: the product is below 2^22, where 1.5 x 2^23 rounds it to an integer)
     const uint64_t i = fma2(y, t8, pair(12582912.f, 12582912.f));
     const uint32_t va = ta.x + ((uint32_t)i - 0x4B400000u) * 8u, vb = tb.x + ((uint32_t)(i >> 32) - 0x4B400000u) * 8u;
-    wa = ((unsigned long long)va << 14) >> (unsigned)-(na >> 6);
-    wb = ((unsigned long long)vb << 14) >> (unsigned)-(nb >> 6);
+    wa = shift_right((unsigned long long)va << 14, -(na >> 6));
+    wb = shift_right((unsigned long long)vb << 14, -(nb >> 6));
     if (band) {  // for a coarse sum by weight: the band of 4^-b, and the weight times 2^28 in fp32
       const uint64_t f = fma2(y, t8, t8);
       band[0] = min(-na >> 7, BANDS - 1);
@@ -669,15 +676,19 @@ __global__ void __launch_bounds__(RT, 2)
   const float T_row = temperature ? temperature[r] : 1.f;
   const float m = K::value(row_top);
   constexpr float LOG2E_1 = 1.442695041f, LOG2E_2 = 1.925963e-8f;  // log2(e) in two parts
-  row.c1 = LOG2E_1 / T_row;
-  row.c2 = (fmaf(-row.c1, T_row, LOG2E_1) + LOG2E_2) / T_row;
-  row.mp = __fmul_rn(m, row.c1);
-  row.me = fmaf(m, row.c1, -row.mp);
-  row.ml = __fmul_rn(m, row.c2);
-  // (a product that overflows, as at temperatures near 0: the largest logit alone has a weight)
-  row.inf = isinf(m) || !(fabsf(row.mp) < 1e37f);
+  // (differences of logits may overflow where they matter, log2(e) / T does at subnormal temperatures)
+  row.scale = T_row > 1e30f ? 0.5f : T_row < 1e-20f ? 18446744073709551616.f : 1.f;
+  const float T_scaled = T_row * row.scale;
+  row.c1 = LOG2E_1 / T_scaled;
+  row.c2 = isinf(T_row) ? 0.f : (fmaf(-row.c1, T_scaled, LOG2E_1) + LOG2E_2) / T_scaled;
+  row.minus = -m * row.scale;
+  // At a temperature below 2^-29 or so of the largest logit, the next lower fp32 number weighs less than
+  // 2^-46: the largest logit alone has a weight.
+  row.inf = isinf(m) || !(fabsf(row.minus) * row.c1 < 7.7e8f);
   row.careful = row.inf || T_row > 1e30f;
-  row.least = fmaxf(m - 41.6f * T_row, -3.4028234663852886e38f);  // (60 ln 2: a weight of 2^-60)
+  row.least = m - 41.6f * T_row;  // (60 ln 2)
+  if (m - row.least < 41.f * T_row) row.least = nextafterf(row.least, -INFINITY);
+  row.least = fmaxf(row.least, -3.4028234663852886e38f);
   // the key of a logit that weighs w, or of one a little lighter (the logarithm's error is a bound's)
   auto key_at = [&](float w) -> uint32_t {
     const float x = m + T_row * (logf(w) - 1e-3f);
@@ -747,7 +758,8 @@ __global__ void __launch_bounds__(RT, 2)
       });
       cl.sync();
       if (rank == 0)
-        draw_from_list(sh, row, (int)n_list, some ? k : 0, tp, floor_w, uniform[r], tokens + r, probs ? probs + r : nullptr);
+        draw_from_list(sh, row, (int)n_list, some ? k : 0, tp, mp > 1.f ? ~0ull : floor_w, uniform[r], tokens + r,
+                       probs ? probs + r : nullptr);
       return;
     }
   }

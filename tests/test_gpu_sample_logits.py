@@ -3,6 +3,8 @@ against the definition in 64 bits on the host: tokens equal, probabilities withi
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -143,6 +145,48 @@ def test_extreme_temperatures(ops, cuda_device) -> None:
     settings = [(1e-6, 0, 1.0, 0.0), (1e-6, 0, 0.9, 0.0), (1e4, 0, 0.5, 0.0), (1e4, 700, 0.5, 0.0), (1e30, 0, 1.0, 0.0),
                 (1e30, 0, 0.3, 0.5)]
     check(ops, logits, settings, u)
+
+
+@pytest.mark.parametrize("temperature", [1e-1, 1e-3, 1e-5, 1e-6, 1e-7, 3e-8, 1e-8, 1e-12, 1e-30, 1e-42])
+@pytest.mark.parametrize("top", [20.0, -37.7, 0.0])
+def test_low_temperatures_beside_near_ties(ops, cuda_device, temperature, top) -> None:
+    """Logits a few units in the last place (or a few temperatures) below the largest one."""
+    g = torch.Generator().manual_seed(int(-math.log10(temperature)))
+    n, vocab = 8, 3000
+    step = max(temperature, np.spacing(np.float32(top)) / 2) if top else temperature
+    near = top - torch.randint(0, 60, (n, vocab), generator=g).double() * step * 0.7
+    logits = torch.where(torch.rand((n, vocab), generator=g) < 0.9, torch.tensor(top - 1.0).double(), near).float()
+    settings = [(temperature, 0, 1.0, 0.0), (temperature, 0, 0.9, 0.0), (temperature, 40, 0.95, 0.01), (temperature, 0, 1.0, 1.0),
+                (temperature, 0, 0.9, 1.0), (temperature, 0, 0.5, 2.0), (temperature, 2000, 0.999, 0.0), (temperature, 0, 1.0, 1e-6)]
+    check(ops, logits.to(cuda_device), settings, torch.rand(n, generator=g).to(cuda_device))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logits_far_from_zero(ops, cuda_device, dtype) -> None:
+    """A shift of all logits changes nothing but what it rounds away."""
+    for shift in (300.0, -4096.0, 1e5, -3e7):
+        logits, u = language_logits(len(SETTINGS), 9000, 31, cuda_device, torch.float32)
+        check(ops, (logits + shift).to(dtype), SETTINGS, u)
+
+
+def test_temperatures_up_to_infinity(ops, cuda_device) -> None:
+    logits, u = language_logits(8, 3000, 41, cuda_device, torch.float32)
+    logits[:, 5::9] = float("-inf")
+    logits[:, 7::50] = torch.finfo(torch.float32).min
+    inf = float("inf")
+    check(ops, logits, [(inf, 0, 1.0, 0.0), (inf, 0, 0.4, 0.0), (inf, 30, 0.5, 0.0), (inf, 0, 1.0, 0.5), (1e31, 0, 0.7, 0.0),
+                        (1e36, 0, 1.0, 0.0), (1e36, 2500, 0.9, 0.0), (1e36, 0, 1.0, 1.0)], u)
+    logits = logits.sign() * 3.3e38  # differences that overflow
+    logits[:, 0] = 3.3e38
+    check(ops, logits, [(1e36, 0, 1.0, 0.0)] * 4 + [(1e36, 0, 0.9, 0.0)] * 4, u)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_min_p_above_one_keeps_one_token(ops, cuda_device, dtype) -> None:
+    logits = torch.zeros((6, 500), dtype=dtype, device=cuda_device)
+    u = torch.linspace(0, 0.99, 6, device=cuda_device)
+    check(ops, logits, [(1.0, 0, 1.0, 1.5), (1.0, 0, 0.9, 1.5), (1.0, 40, 1.0, 1.5), (0.5, 40, 0.5, 7.0), (1.0, 400, 0.9, 1.1),
+                        (1.0, 0, 1.0, float("inf"))], u)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
