@@ -337,14 +337,16 @@ class B200SpeculativeEngine:
             shared = int(self.state.num_shared_blocks[slots[0]].item())
             self._fork_blocks.update((s, shared) for s in slots)
         self._dev_slots_key = None  # (the same slots may now hold other sequences)
+        holder = slot if slot in self._prefixes else self._prefix_of.get(slot)
         for s in slots:
             self._uncached[s] = 1
             self._fork_of[s] = slot
-            if slot in self._prefix_of:  # the prefix's blocks are theirs as well
-                self._prefix_of[s] = self._prefix_of[slot]
-                self._prefixes[self._prefix_of[slot]][2] += 1
+            if holder is not None:  # the prefix's blocks are theirs as well
+                self._prefix_of[s] = holder
+                self._prefixes[holder][2] += 1
+                blocks = self._prefixes[holder][1] if slot == holder else self._shared_count[slot]
                 # (a fork cut inside the prefix shares the full blocks before its last token)
-                self._shared_count[s] = min(self._shared_count[slot], (at - 1) // 16 if at else 1 << 30)
+                self._shared_count[s] = min(blocks, (at - 1) // 16 if at else 1 << 30)
         return slots
 
     def trim(self, slots: list[int]) -> None:

@@ -159,6 +159,29 @@ def test_a_fork_cut_inside_the_prefix(pkg, make, at) -> None:
     assert n >= 4 and outs[True][1][:n] == want[:n] and outs[True][2] == outs[True][1]
 
 
+@pytest.mark.parametrize("on", [False, True], ids=["plain", "shared"])
+def test_forks_of_a_prefix_itself_keep_it(pkg, make, on) -> None:
+    """Forks of the handle that ``add_prefix`` gives are users of the prefix."""
+    prompt = prompts_with_prefix(pkg, 160, 1)[0]
+    eng = make(shared=on)
+    holder = eng.add_prefix(prompt[:150])
+    slots = eng.fork(holder, 2, at=140) + [eng.add_request(prompt, 8, ignore_eos=True, prefix=holder)]
+    with pytest.raises(RuntimeError):
+        eng.drop_prefix(holder)
+    eng.state.max_new_tokens[torch.tensor(slots[:2], device=eng.model.device)] = 8
+    res = eng.prefill(slots)
+    out = {s: list(res.tokens[s]) for s in slots}
+    while len(out[slots[2]]) < 8:
+        for s, t in eng.step(slots).tokens.items():
+            out[s] += t
+    plain = make(shared=False)
+    want = [plain.generate([p], 8)[0] for p in (prompt[:140], prompt[:140], prompt)]
+    assert [out[s][:8] for s in slots] == want
+    eng.release(slots)
+    eng.drop_prefix(holder)
+    assert eng.state.num_free_blocks() == 192
+
+
 def test_fork_step_and_sample_by_hand(pkg, make, cuda_device) -> None:
     """A user's own loop: prefill, fork, one step, and next tokens drawn from the step's logits with
     top-k, top-p and min-p; the draw equals the definition on those logits."""
