@@ -985,9 +985,13 @@ int launch_sample_rows(const void* logits, int rows, int vocab, long long row_st
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   // Slices of up to 80 KB, two CTAs an SM: the barriers of a larger cluster cost more than its shorter
   // slices save (measured, 320 rows of 151,936 bf16, top-k 20: 2 / 4 / 8 CTAs 97 / 79 / 123 us). Few rows
-  // leave SMs idle, and slices above 8,192 tokens are halved then.
+  // leave SMs idle, and slices above 8,192 tokens are halved then; where every SM has one CTA, above
+  // 14,000 (measured, rows of mixed settings: slices of 16,000 / 19,000 / 20,000 tokens halved take 60 -> 47,
+  // 125 -> 90 and 70 -> 55 us, of 12,500 58 -> 67).
   while (ctas < MAX_CLUSTER && (size_t)vocab * sizeof(T) > (80u << 10) * ctas) ctas *= 2;
-  while (ctas < MAX_CLUSTER && vocab > 8192 * ctas && 2LL * rows * ctas <= sms) ctas *= 2;
+  while (ctas < MAX_CLUSTER && (long long)rows * ctas <= sms &&
+         vocab > (2LL * rows * ctas <= sms ? 8192 : 14000) * ctas)
+    ctas *= 2;
   const int slice = (vocab + ctas - 1) / ctas;
   const size_t smem = ((size_t)slice * sizeof(T) + 47) / 16 * 16;  // (a padded vector at either end)
   if (smem > MAX_SLICE_BYTES) return NE_ERR_UNSUPPORTED;
