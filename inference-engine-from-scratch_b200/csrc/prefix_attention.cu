@@ -564,6 +564,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -699,6 +706,15 @@ struct Walk {
     return false;
   }
 };
+
+// Two int8 values of ``word`` as bf16, exact: with its sign bit s and the seven others v, a value is
+// (128 + v) - (s ? 256 : 128), both of which are bf16 numbers with the byte as their low bits.
+__device__ __forceinline__ uint32_t exact_pair(uint32_t word, uint32_t sel) {
+  const uint32_t p = __byte_perm(word, 0x43434343u, sel);
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(p & 0x437F437Fu), "r"(p & 0x43804380u));
+  return d;
+}
 
 template <bool INT8>
 __global__ void __launch_bounds__(pre_threads(INT8), 1)
@@ -888,40 +904,57 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
         const int t = j >> 1, half = j & 1;  // are computed while this one's weights are
         ok = mbar_wait(&sh.s_full[s][half], (tiles_before + t) & 1u, &sh.abort_flag, status);
         tc_fence_after();
-        float x[HALF];
-        tmem_ld32_start(t_s + HALF * half, x);
-        tmem_ld32_start(t_s + HALF * half + 32, x + 32);
+        // int8: 32 keys at a time, the second 32 loaded twice (their maximum, then their weights), for the
+        // scales take registers and what is spilled does not fit what shared memory leaves of the L1
+        constexpr int KEYS = INT8 ? HALF / 2 : HALF;
+        float x[KEYS];
+        tmem_ld32_start(t_s + HALF * half + (INT8 ? KEYS : 0), x);
+        if (!INT8) tmem_ld32_start(t_s + HALF * half + 32, x + 32 % KEYS);
         // the mask comes with the V tile (K's slot may be refilled by now)
         const uint32_t v_at = 2 * (slots_before + t) + 1;
         ok = ok && mbar_wait(&sh.full[v_at % RING], (v_at / RING) & 1u, &sh.abort_flag, status);
         const uint32_t valid = sh.valid[v_at % RING] >> (4 * half) & 0xFu;
-        tmem_ld_wait();
         const float* scale_k = sh.scale[(v_at % RING) >> 1][0] + HALF * half;
         const float* scale_v = sh.scale[(v_at % RING) >> 1][1] + HALF * half;
-        if (INT8) {
+        auto finish = [&](int k0) {  // the scores of keys k0 .. of the half have been asked for
+          tmem_ld_wait();
+          if (INT8) {
 #pragma unroll
-          for (int c = 0; c < HALF; c += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(scale_k + c);
-            unpack2(mul2(pack2(x[c], x[c + 1]), pack2(k4.x, k4.y)), x[c], x[c + 1]);
-            unpack2(mul2(pack2(x[c + 2], x[c + 3]), pack2(k4.z, k4.w)), x[c + 2], x[c + 3]);
+            for (int c = 0; c < KEYS; c += 4) {
+              const float4 k4 = *reinterpret_cast<const float4*>(scale_k + k0 + c);
+              unpack2(mul2(pack2(x[c], x[c + 1]), pack2(k4.x, k4.y)), x[c], x[c + 1]);
+              unpack2(mul2(pack2(x[c + 2], x[c + 3]), pack2(k4.z, k4.w)), x[c + 2], x[c + 3]);
+            }
           }
+          if (valid != 0xFu) {
+#pragma unroll
+            for (int c = 0; c < KEYS; ++c)
+              if (!(valid >> ((k0 + c) >> 4) & 1u)) x[c] = NEG_INF;
+          }
+        };
+        auto largest = [&] {
+          float mx[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx[i] = max3(x[i], x[8 + i], x[16 + i]);
+#pragma unroll
+          for (int c = 24; c + 16 <= KEYS; c += 16)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx[i] = max3(mx[i], x[c + i], x[c + 8 + i]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx[i] = max2(mx[i], x[KEYS - 8 + i]);
+          return max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max2(mx[6], mx[7]));
+        };
+        float top;
+        if (INT8) {
+          finish(KEYS);
+          top = largest();
+          tmem_ld32_start(t_s + HALF * half, x);
+          finish(0);
+          top = max2(top, largest());
+        } else {
+          finish(0);
+          top = largest() * SCALE_LOG2;
         }
-        if (valid != 0xFu) {
-#pragma unroll
-          for (int c = 0; c < HALF; ++c)
-            if (!(valid >> (c >> 4) & 1u)) x[c] = NEG_INF;
-        }
-        float mx[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx[i] = max3(x[i], x[8 + i], x[16 + i]);
-#pragma unroll
-        for (int c = 24; c < 56; c += 16)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mx[i] = max3(mx[i], x[c + i], x[c + 8 + i]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx[i] = max2(mx[i], x[56 + i]);
-        const float top =
-            max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max2(mx[6], mx[7])) * (INT8 ? 1.f : SCALE_LOG2);
         const bool odd = __any_sync(ALL, !(fabsf(top) < INFINITY));  // NaN or infinite scores among them
         // the reference moves only when the scores pass it by 2^8 (the sums stay far inside fp32)
         if (__any_sync(ALL, !(top <= ref + RESCALE))) {
@@ -946,10 +979,10 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
         const float base = ref == NEG_INF ? 0.f : ref;
         const uint64_t scale2 = pack2(SCALE_LOG2, SCALE_LOG2), base2 = pack2(-base, -base);
         uint64_t sum[2] = {0ull, 0ull};  // (pairs of fp32 zeros)
-        uint32_t p[HALF / 2];
-        auto weigh = [&](bool all) {
+        uint32_t p[KEYS / 2];
+        auto weigh = [&](bool all, int k0) {
 #pragma unroll
-          for (int i = 0; i < HALF / 2; ++i) {
+          for (int i = 0; i < KEYS / 2; ++i) {
             float a, b;
             const uint64_t x2 = pack2(x[2 * i], x[2 * i + 1]);
             const uint64_t t2 = INT8 ? add2(x2, base2) : fma2(x2, scale2, base2);  // (int8: scaled already)
@@ -962,15 +995,24 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
             }
             sum[i & 1] = add2(sum[i & 1], pack2(a, b));
             if (INT8) {
-              const float2 v2 = *reinterpret_cast<const float2*>(scale_v + 2 * i);
+              const float2 v2 = *reinterpret_cast<const float2*>(scale_v + k0 + 2 * i);
               unpack2(mul2(pack2(a, b), pack2(v2.x, v2.y)), a, b);
             }
             p[i] = pack_bf16(a, b);
           }
         };
-        if (odd) weigh(true);
-        else weigh(false);
-        tmem_st32(t_s + HALF * half, p);
+        if (odd) weigh(true, 0);
+        else weigh(false, 0);
+        if constexpr (INT8) {  // (the first keys' weights lie where their scores did)
+          tmem_st16(t_s + HALF * half, p);
+          tmem_ld32_start(t_s + HALF * half + KEYS, x);
+          finish(KEYS);
+          if (odd) weigh(true, KEYS);
+          else weigh(false, KEYS);
+          tmem_st16(t_s + HALF * half + KEYS / 2, p);
+        } else {
+          tmem_st32(t_s + HALF * half, p);
+        }
         float s0, s1;
         unpack2(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
@@ -1210,8 +1252,8 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
           uint32_t o[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            o[2 * k] = dq_pair(w[k], 0x4140u, 0x3F803F80u);
-            o[2 * k + 1] = dq_pair(w[k], 0x4342u, 0x3F803F80u);
+            o[2 * k] = exact_pair(w[k], 0x4140u);
+            o[2 * k + 1] = exact_pair(w[k], 0x4342u);
           }
           uint8_t* row = dst + (ch >> 2) * (SLOT_BYTES / 2) + key * 128;
           *reinterpret_cast<uint4*>(row + (((2 * ch & 7) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
