@@ -107,7 +107,7 @@ __device__ __forceinline__ float max2(float a, float b) {
 // ---------------------------------------------------------------- prefixes: the division of the work
 // A group's vectors of one KV head are cut into items of up to 256: one or two query tiles, which share
 // every tile of 128 keys. A key tile costs an item 3 units of work with one query tile and 4 with two
-// (measured: about 1,900 and 2,500 cycles). The units of all (group, head, item) in turn are divided
+// (measured, bf16: 3,000 and 4,000 cycles; int8, bound by the conversion: 6,900 and 7,400). The units of all (group, head, item) in turn are divided
 // evenly over the CTAs: CTA c does the key tiles that start in its ceil(W / CTAs) units from
 // c ceil(W / CTAs) on.
 __device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 7) / 8; }
@@ -329,7 +329,12 @@ constexpr size_t own_smem() {
 }
 static_assert((2 * 4 * 16 * D + 2 * 2 * 4 * 16) * 4 <= 4 * 4 * BLOCK_BYTES, "merge area");
 
-// Bound by memory: each block is read once per CTA, a CTA's first loads go out before its query tile.
+// Each block is read once per CTA, a CTA's first loads go out before its query tile. Bound by the latency
+// of a warp's own chain: a block takes it 1,300 to 1,700 cycles (QK products, maximum, weights, PV) and
+// 600 to 900 to issue its loads, for which it then waits 60 at most; the CTA's first loads come 6,000
+// cycles after its start (entry, positions, table). 256 entries of 100 own tokens on average and 8 KV heads,
+// alone and from DRAM: 39 us, 115 MB. Three or four stages a warp, two blocks a softmax step, heads as the
+// fastest grid axis, and CTAs beside prefix_kernel's (which then slows as much) were measured: none is faster.
 template <bool INT8, int NW, int NT>
 __global__ void __launch_bounds__(32 * NW * NT, NT == 2 ? 2 : NW == 8 ? 1 : NW == 4 ? 3 : 5)
     own_tokens_kernel(const __nv_bfloat16* __restrict__ q, const void* __restrict__ kc, const void* __restrict__ vc,
@@ -716,6 +721,14 @@ __device__ __forceinline__ uint32_t exact_pair(uint32_t word, uint32_t sel) {
   return d;
 }
 
+// Per segment, S = Q K^T (Q, K in shared memory, S in TMEM), P = 2^(S - ref) in S's columns, O += P V (P from
+// TMEM), 64 keys a step so that the tensor cores work on one half's products while the other's weights
+// are computed; O is rescaled only when the reference moves by more than 2^8. K and V tiles come through
+// a ring of four slots by 3-D tensor loads of the 16-token pages (int8: loaded and converted by four
+// warps). Bound by the softmax's instructions: 16,384 shared tokens x 1,280 vectors x 8 KV heads (85.9
+// GFLOP) take 103 us, 834 TFLOP/s, with the tensor pipe busy 47% of the time (a pair tile's products alone
+// are 2,048 of its 4,000 cycles); 3 of 8 powers of two run on the FMA pipe. A CTA's
+// fixed costs are about 15,000 cycles: plan 6,000, first query tile 2,700, epilogue 3,500 a segment.
 template <bool INT8>
 __global__ void __launch_bounds__(pre_threads(INT8), 1)
     prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -1282,7 +1295,8 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
 constexpr int JOIN_WARPS = 8;
 
 // A warp per vector. Bound by latency: three loads in a row behind the wait (where the parts are,
-// their sums of weights, their values), the inputs before it.
+// their sums of weights, their values), the inputs before it. 20,480 vectors of two to three parts (31 MB,
+// which lie in L2 behind the other two launches): 21 us alone and from DRAM.
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
     join_kernel(__nv_bfloat16* __restrict__ out, ne_rows rows, ne_prefix_groups groups, int nh, int nkv, Parts parts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.y;

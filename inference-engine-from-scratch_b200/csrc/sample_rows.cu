@@ -15,6 +15,12 @@
 // decided by sums over the whole vocabulary, so weights are good to about 2e-9 (an error of 1e-7, as
 // plain fp32 gives, moves the border of a flat distribution past a token) and summed in steps of 2^-45,
 // whose sums do not depend on their order: the same inputs give the same tokens.
+//
+// Where a lower bound of all cuts (from the quarter warps' maxima, or min-p) leaves at most 2,048 tokens,
+// they are gathered and sorted by one CTA; else the cuts are selected over the row. Bound by instructions
+// (2 of 4 issue slots used), not by the 97 MB: 320 rows of 151,936 bf16 logits take 33 us greedy, 67 to 87
+// with top-k or min-p, 131 without a filter, 265 with top-p 0.9 at temperature 0.8 and 660 with top-p 0.999
+// at 1.5 (every third token a candidate), 228 with all of these mixed; one row 14 to 73.
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"
