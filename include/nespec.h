@@ -544,7 +544,9 @@ NE_API int ne_model_set_prefix_groups(ne_model* model, const ne_prefix_groups* g
  * the argmax (lowest id), probability 1. temperature, top_k, top_p and min_p are [rows] device
  * arrays or NULL (1, 0, 1 and 0 for every row). NaN and -inf logits are never drawn; a row of only
  * those gives token -1, probability 0 and NE_DEV_BAD_TOKEN. If a logit is +inf, the mass lies on
- * those that are. Sums are exact in fixed point: equal inputs give equal tokens. vocab <= 262144.
+ * those that are. Sums are exact in fixed point (steps of 2^-45 of the largest weight, weights good to
+ * about 2e-9; a border nearer to a token than that may leave it out): equal inputs give equal tokens.
+ * vocab <= 262144.
  */
 NE_API int ne_sample_logits(const void* logits, int logits_fp32, int rows, int vocab, long long row_stride,
                             const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,

@@ -18,9 +18,9 @@
 //
 // Where a lower bound of all cuts (from the quarter warps' maxima, or min-p) leaves at most 2,048 tokens,
 // they are gathered and sorted by one CTA; else the cuts are selected over the row. Bound by instructions
-// (2 of 4 issue slots used), not by the 97 MB: 320 rows of 151,936 bf16 logits take 33 us greedy, 67 to 87
-// with top-k or min-p, 131 without a filter, 265 with top-p 0.9 at temperature 0.8 and 660 with top-p 0.999
-// at 1.5 (every third token a candidate), 228 with all of these mixed; one row 14 to 73.
+// (2 of 4 issue slots used), not by the 97 MB: 320 rows of 151,936 bf16 logits take 41 us greedy, 72 to 92
+// with top-k or min-p, 135 without a filter, 270 with top-p 0.9 at temperature 0.8 and 670 with top-p 0.999
+// at 1.5 (every third token a candidate), 176 with all of these mixed; one row 14 to 73.
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"
@@ -601,9 +601,50 @@ __device__ void draw_from_list(Shared& sh, const Row<T>& row, int n, int k, floa
   }
 }
 
+// The row of cluster ``place``: the rows whose cuts are selected over the whole row first, each kind in
+// ascending order. They take up to ten times the others, and one that starts last holds the launch.
+__device__ int row_at(Shared& sh, int place, int rows, int listed, const float* temperature, const int32_t* top_k,
+                      const float* top_p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto slow = [&](int r) {  // (the three loads side by side)
+    r = min(r, rows - 1);
+    const float p = top_p[r], t = temperature ? temperature[r] : 1.f;
+    const int k = top_k ? top_k[r] : 0;
+    return p < 1.f & t > 0.f & !(k > 0 & k <= listed);
+  };
+  int many = 0;
+  bool mine = slow(threadIdx.x);
+  uint32_t votes = __ballot_sync(ALL, mine & threadIdx.x < rows);
+  if (lane == 0) sh.red32[warp] = __popc(votes);
+  __syncthreads();
+  for (int w = 0; w < RW; ++w) many += sh.red32[w];
+  for (int r0 = RT; r0 < rows; r0 += RT) many += __syncthreads_count(slow(r0 + threadIdx.x) & r0 + threadIdx.x < rows);
+  const bool want = place < many;
+  int before = want ? 0 : many;
+  for (int r0 = 0; r0 < rows; r0 += RT) {
+    const int r = r0 + threadIdx.x;
+    if (r0 > 0) mine = slow(r);
+    mine = (mine == want) & r < rows;
+    votes = __ballot_sync(ALL, mine);
+    __syncthreads();
+    if (lane == 0) sh.red32[warp] = __popc(votes);
+    __syncthreads();
+    int at = before + __popc(votes & ((1u << lane) - 1u));
+    for (int w = 0; w < RW; ++w) {
+      if (w < warp) at += sh.red32[w];
+      before += sh.red32[w];
+    }
+    if (mine & at == place) sh.pub_id = r;
+  }
+  __syncthreads();
+  const int row = sh.pub_id;
+  __syncthreads();
+  return row;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(RT, 2)
-    sample_rows_kernel(const T* __restrict__ logits, long long row_stride, int vocab, int slice,
+    sample_rows_kernel(const T* __restrict__ logits, long long row_stride, int vocab, int slice, int ordered_rows,
                        const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
                        const float* __restrict__ top_p, const float* __restrict__ min_p,
                        const float* __restrict__ uniform, int32_t* __restrict__ tokens,
@@ -615,7 +656,8 @@ __global__ void __launch_bounds__(RT, 2)
   extern __shared__ __align__(16) uint8_t slice_smem[];
   cg::cluster_group cl = cg::this_cluster();
   const int ctas = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  const int r = blockIdx.x / ctas;
+  int r = blockIdx.x / ctas;
+  if (ordered_rows > 0) r = row_at(sh, r, ordered_rows, 4 * RW * ctas, temperature, top_k, top_p);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = min(vocab, rank * slice), n = min(vocab, first + slice) - first;
   if (tid < 64) sh.pow2[tid] = make_uint2(POW2[tid], __float_as_uint((float)POW2[tid] * 0.125f));
@@ -1000,6 +1042,9 @@ int launch_sample_rows(const void* logits, int rows, int vocab, long long row_st
     ctas *= 2;
   const int slice = (vocab + ctas - 1) / ctas;
   const size_t smem = ((size_t)slice * sizeof(T) + 47) / 16 * 16;  // (a padded vector at either end)
+  // rows that do not all start at once are put in order (320 rows of mixed settings 228 -> 176 us; of one
+  // setting, where the order gains nothing, 33 -> 41 to 660 -> 670)
+  const int ordered = top_p && (long long)rows * ctas > 2LL * sms && rows <= 4096 ? rows : 0;
   if (smem > MAX_SLICE_BYTES) return NE_ERR_UNSUPPORTED;
   static bool done[64] = {};
   if (!done[dev]) {
@@ -1019,7 +1064,7 @@ int launch_sample_rows(const void* logits, int rows, int vocab, long long row_st
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = add_common_attrs(attr, 1);
-  return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, static_cast<const T*>(logits), row_stride, vocab, slice,
+  return cudaLaunchKernelEx(&cfg, sample_rows_kernel<T>, static_cast<const T*>(logits), row_stride, vocab, slice, ordered,
                             temperature, top_k, top_p, min_p, uniform, tokens, probs, status) == cudaSuccess
              ? NE_OK
              : NE_ERR_CUDA;
