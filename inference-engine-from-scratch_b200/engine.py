@@ -737,7 +737,8 @@ class B200SpeculativeEngine:
                          temperature: float = 1.0, top_p: float = 1.0, seeds: list[int] | None = None,
                          prefill_chunk: int | None = None) -> list[list[int]]:
         """``n`` completions of one prompt (sample i on ``seeds[i]``, default i), which is prefilled
-        once: the others are forks that share its blocks, each with a first token of its own."""
+        once: the others are forks that share its blocks, each with a first token of its own. All samples
+        run together: a pool that cannot hold them ends the call with its error, and they are released."""
         if n < 1 or n > self.max_seqs:
             raise ValueError(f"between 1 and max_seqs = {self.max_seqs} samples")
         seeds = list(seeds) if seeds is not None else list(range(n))
@@ -757,6 +758,11 @@ class B200SpeculativeEngine:
             while any(f is None for f in finish):
                 running = [i for i in range(n) if finish[i] is None]
                 res = self.step([slots[i] for i in running])
+                if not all(res.tokens[slots[i]] for i in running):
+                    # a sequence that runs gets a token from every step, unless its blocks did not fit;
+                    # such a step changes nothing, and the next one would not fit either
+                    self.model.raise_on_device_error()
+                    raise RuntimeError("a step yielded no token for a running sample")
                 for i in running:
                     outputs[i].extend(res.tokens[slots[i]])
                     finish[i] = res.finish[slots[i]]

@@ -269,6 +269,20 @@ def test_samples_of_one_prompt(pkg, make_engine, kv_int8, length) -> None:
     assert greedy == make_engine(kv_int8).generate([prompt], 16) * 3
 
 
+@pytest.mark.parametrize("num_blocks", [2, 8, 12, 20])
+def test_samples_that_outgrow_the_pool_end_with_an_error(pkg, make_engine, num_blocks) -> None:
+    """The pool runs out in the prompt's prefill, in the forks' or in a step: the call raises, every slot
+    and block is back, and samples that fit are served as ever."""
+    eng = make_engine(num_blocks=num_blocks)
+    prompt = pkg.make_prompt(pkg.SMALL_TEST.vocab_size, 33, 4, False)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="out of KV blocks"):
+            eng.generate_samples(prompt, 8, 200, temperature=0.8)
+        assert eng.state.num_free_blocks() == num_blocks and len(eng.state.free_slots) == 8
+    if num_blocks >= 8:  # (33 + 10 tokens and 4 guesses: three blocks of which two are shared)
+        assert [len(t) for t in eng.generate_samples(prompt, 2, 10, temperature=0.8)] == [10, 10]
+
+
 @pytest.mark.parametrize("kv_int8", [False, True], ids=["bf16", "int8"])
 def test_a_fork_on_the_same_stream_draws_what_its_source_draws(pkg, make_engine, kv_int8) -> None:
     """Forked with all its tokens and without seeds, a sequence holds its source's very state: in one
