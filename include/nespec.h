@@ -525,7 +525,7 @@ NE_API int ne_prefix_attention(const void* q, void* out, const void* k_cache, co
 /*
  * Let the model's steps use ne_prefix_attention in place of ne_paged_attention: forwards of up to 32
  * query vectors per entry and KV head (speculative steps, single tokens) whose bounds fit the
- * workspace; longer ones (prefills) keep the ordinary attention. The arrays are read by every such
+ * workspace and ne_prefix_attention's limits; others (prefills) run as they do without groups. The arrays are read by every such
  * forward: entry_group [at least the forward's num_seqs] names the batch entries' groups, so a captured
  * step follows their contents. groups NULL (or num_groups 0): off.
  */

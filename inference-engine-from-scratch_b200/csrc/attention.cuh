@@ -46,8 +46,11 @@ int launch_attention_tc(const __nv_bfloat16* q, __nv_bfloat16* out, const void* 
                         const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8, const ne_rows& rows,
                         int num_heads, int num_kv_heads, long long num_cache_slots, const AttnSplit& sp, int* status,
                         cudaStream_t stream, const KvShadow& shadow = KvShadow{});
-// Attention over prompt prefixes that groups of entries share (prefix_attention.cu); NE_ERR_WORKSPACE when
-// ``ws`` (256-byte aligned) is too small for the launch's bounds.
+// Attention over prompt prefixes that groups of entries share (prefix_attention.cu). prefix_attention_fits is
+// NE_OK for the bounds that a launch can serve with ``ws_bytes`` of workspace (256-byte aligned); the launch
+// returns its error otherwise.
+int prefix_attention_fits(const ne_rows& rows, const ne_prefix_groups& groups, int num_heads, int num_kv_heads,
+                          size_t ws_bytes);
 int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const void* k_cache, const void* v_cache,
                             const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8,
                             const ne_rows& rows, ne_prefix_groups groups, int num_heads, int num_kv_heads,

@@ -699,7 +699,13 @@ int ne_forward(ne_model* m, const ne_rows* rows, int lm_mode, void* logits, int3
   if (lm_mode == NE_LM_LOGITS && !logits) return NE_ERR_INVALID;
   const bool tp = m->tp_world > 1;
   if (tp && lm_mode == NE_LM_LOGITS) return NE_ERR_UNSUPPORTED;  // logits are split over the ranks
-  if (m->prefix.num_groups == 0 && use_step_kernel(m, rows, lm_mode)) return step_forward(m, rows, argmax_out, as_stream(stream));
+  const int group = c.num_heads / c.num_kv_heads;
+  const int max_vec = std::max(1, rows->max_q_len) * group;
+  // steps of up to two query tiles an entry read the prefixes that their entries share once, where
+  // their bounds fit; any other forward runs as it does without groups
+  const bool shared = m->prefix.num_groups > 0 && max_vec <= 32 &&
+                      ne::prefix_attention_fits(*rows, m->prefix, c.num_heads, c.num_kv_heads, m->prefix_ws_bytes) == NE_OK;
+  if (!shared && use_step_kernel(m, rows, lm_mode)) return step_forward(m, rows, argmax_out, as_stream(stream));
   // a split model exchanges partial rows through peer memory when they fit the exchange slots
   // (every rank takes the same branch: R and lm_max are the same host values on all ranks)
   const bool px = tp && m->link.world > 0 && R <= m->link.max_rows && rows->lm_max <= m->link.max_rows;
@@ -718,17 +724,10 @@ int ne_forward(ne_model* m, const ne_rows* rows, int lm_mode, void* logits, int3
                 ne::launch_embed(embed, rows->token_ids, rows->num_rows, R, H, c.vocab_size, m->h, m->status, s,
                                  fuse ? m->ssq : nullptr), s);
   if (rc) return rc;
-  const int group = c.num_heads / c.num_kv_heads;
-  const int max_vec = std::max(1, rows->max_q_len) * group;
   const int splits = ne::attention_plan_splits(rows->num_seqs, c.num_kv_heads, rows->max_context, max_vec,
                                                m->num_sms, m->attn_scratch_bytes);
   const ne::AttnSplit attn = ne::attention_split_view(m->attn_scratch, (long long)rows->num_seqs * c.num_kv_heads,
                                                       splits, max_vec);
-  // steps of up to two query tiles an entry read the prefixes that their entries share once
-  const bool shared = m->prefix.num_groups > 0 && max_vec <= 32 &&
-                      ne_prefix_attention_workspace_bytes(R, rows->num_seqs, m->prefix.num_groups, c.num_heads,
-                                                          c.num_kv_heads, std::max(1, rows->max_q_len),
-                                                          rows->max_context) <= m->prefix_ws_bytes;
   // rows the RMSNorm loads before reading the device row count: a speculative step's expected
   // rows plus a quarter (the bucket's bound is far above them: loading every row of it cost config
   // 4, 1,280 rows for ~500, 7.53 -> 7.95 ms per step)

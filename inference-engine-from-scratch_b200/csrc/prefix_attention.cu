@@ -1345,21 +1345,35 @@ bool heads_ok(int nh, int nkv) { return nkv > 0 && nh > 0 && nh % nkv == 0 && nh
 
 }  // namespace
 
-int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const void* k_cache, const void* v_cache,
-                            const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8,
-                            const ne_rows& rows, ne_prefix_groups groups, int nh, int nkv, long long slots,
-                            uint8_t* ws, size_t ws_bytes, int* status, cudaStream_t stream) {
-  const int sms = device_sms(), G = nh / nkv;
-  const int chunks = own_chunks(rows.max_q_len, G);
+// Whether a launch within these bounds can run: the entries and groups that the plan's arrays have places for,
+// the grids' limits, rows of an entry in 20 bits and units of work in 31, and the workspace.
+int prefix_attention_fits(const ne_rows& rows, const ne_prefix_groups& groups, int nh, int nkv, size_t ws_bytes) {
+  if (rows.num_seqs < 1 || rows.num_seqs > MAX_SEQS || groups.num_groups < 0 || groups.num_groups > MAX_SEQS ||
+      rows.max_rows < 1 || rows.max_q_len < 1 || rows.max_context < 0 || groups.max_prefix_blocks < 0 ||
+      !heads_ok(nh, nkv))
+    return NE_ERR_INVALID;
+  const int sms = device_sms(), chunks = own_chunks(rows.max_q_len, nh / nkv);
   const int splits = own_splits(rows.num_seqs, nkv, chunks, rows.max_context, sms);
-  const Layout l = layout_of(rows.max_rows, rows.num_seqs, groups.num_groups, nh, splits, sms);
-  if (ws_bytes < l.total) return NE_ERR_WORKSPACE;
-  // grid limits; rows of an entry in 20 bits, and units of work in 31
+  if (ws_bytes < layout_of(rows.max_rows, rows.num_seqs, groups.num_groups, nh, splits, sms).total)
+    return NE_ERR_WORKSPACE;
   if ((long long)chunks * splits > 65535 || nkv > 65535 || rows.max_q_len >= (1 << 20) ||
       (long long)rows.max_rows * nh >= (1 << 29) ||
       ((long long)rows.max_rows * nh / TILE + 2LL * groups.num_groups * nkv + 2) * (groups.max_prefix_blocks / 8 + 1) >=
           (1 << 28))
     return NE_ERR_UNSUPPORTED;
+  return NE_OK;
+}
+
+int launch_prefix_attention(const __nv_bfloat16* q, __nv_bfloat16* out, const void* k_cache, const void* v_cache,
+                            const __nv_bfloat16* k_scale, const __nv_bfloat16* v_scale, int kv_int8,
+                            const ne_rows& rows, ne_prefix_groups groups, int nh, int nkv, long long slots,
+                            uint8_t* ws, size_t ws_bytes, int* status, cudaStream_t stream) {
+  const int fits = prefix_attention_fits(rows, groups, nh, nkv, ws_bytes);
+  if (fits != NE_OK) return fits;
+  const int sms = device_sms(), G = nh / nkv;
+  const int chunks = own_chunks(rows.max_q_len, G);
+  const int splits = own_splits(rows.num_seqs, nkv, chunks, rows.max_context, sms);
+  const Layout l = layout_of(rows.max_rows, rows.num_seqs, groups.num_groups, nh, splits, sms);
   if (groups.max_prefix_blocks == 0) groups.num_groups = 0;
   auto f = [&](size_t at) { return reinterpret_cast<float*>(ws + at); };
   const Parts parts{f(l.own_o), f(l.own_m), f(l.own_l), f(l.pre_o), f(l.pre_m), f(l.pre_l),

@@ -229,6 +229,26 @@ def test_the_model_keeps_no_groups_between_launches(pkg, make, graphs) -> None:
     eng.release(slots)
 
 
+def test_groups_whose_bounds_cannot_be_served_leave_steps_as_they_are(pkg, make, cuda_device) -> None:
+    """Bounds past the shared attention's limits (here its units of work) are a forward without groups,
+    not a failed one."""
+    _lib = submodule("_lib")
+    prompts = prompts_with_prefix(pkg, 60, 3)
+    want = make(shared=False).generate(prompts, 10)
+    eng = make(shared=False)
+    entry_group = torch.full((16,), -1, dtype=torch.int32, device=cuda_device)
+    prefix_blocks = torch.ones(16, dtype=torch.int32, device=cuda_device)
+    ws = torch.zeros(64 << 20, dtype=torch.uint8, device=cuda_device)
+    groups = _lib.PrefixGroups(num_groups=16, max_prefix_blocks=1 << 30, entry_group=entry_group.data_ptr(),
+                               prefix_blocks=prefix_blocks.data_ptr())
+    assert eng.lib.ne_model_set_prefix_groups(eng.model.handle, ctypes.byref(groups), ws.data_ptr(), ws.numel()) == 0
+    try:
+        assert eng.generate(prompts, 10) == want
+    finally:
+        eng.lib.ne_model_set_prefix_groups(eng.model.handle, None, None, 0)
+    assert torch.count_nonzero(ws) == 0
+
+
 def test_model_entry_refuses_bad_arguments(pkg, make, cuda_device) -> None:
     _lib = submodule("_lib")
     eng = make()
