@@ -54,6 +54,9 @@ constexpr unsigned long long ONE = 1ull << 45;    // a weight of 1
 constexpr int MAX_VOCAB = 1 << 18;        // 262,144 weights of at most 1 sum to at most 2^63
 constexpr size_t MAX_SLICE_BYTES = 132 << 10;  // MAX_VOCAB / MAX_CLUSTER tokens in fp32, and a padded vector
 static_assert((MAX_SLICE_BYTES / 16 + RW - 1) / RW <= 32 * MOST_CHUNKS, "a warp's chunks");
+constexpr size_t MID_SLICE_BYTES = 80 << 10;  // largest slice of clusters below the largest (launch_sample_rows)
+constexpr int MOST_SLICE = MID_SLICE_BYTES / 2 > MAX_VOCAB / MAX_CLUSTER ? MID_SLICE_BYTES / 2 : MAX_VOCAB / MAX_CLUSTER;
+static_assert((unsigned long long)MOST_SLICE << 15 <= 0xFFFFFFFFull, "pieces of a bin");
 
 // Ordered key of a logit, in the low bits: 16 for bf16, 32 for fp32. NaN and -inf: never drawn.
 // A vector is 16 bytes of a row; ``top`` is its largest logit (NaN aside).
@@ -119,8 +122,8 @@ struct Keys<float> {
   using Raw = uint32_t;
 };
 
-// Fixed-point masses of a bin in three 15-bit pieces: a CTA's 2^15 tokens of at most 2^45 add up in 32
-// bits each, by the 32-bit shared-memory atomics (a 64-bit one took a pass from 15 to 90 us a row).
+// Fixed-point masses of a bin in three 15-bit pieces (the upper one up to 2^15): those of a CTA's 40,960
+// tokens at most add up in 32 bits each, by the 32-bit shared-memory atomics (a 64-bit one took a pass from 15 to 90 us a row).
 struct Bins {
   uint32_t count[BINS], piece[3][BINS];
 };
@@ -128,7 +131,8 @@ struct Bins {
 struct List {
   unsigned long long entry[MOST], mass[MOST];
 };
-struct Shared {
+// (The slice lies behind it: begun 16 bytes past a 32-byte boundary, 320 rows of 151,936 take 4 us more.)
+struct alignas(128) Shared {
   union {
     Bins bins[2];
     List list;
@@ -149,8 +153,6 @@ struct Shared {
   int sel_bin;
   uint32_t sel_count;
   unsigned long long sel_mass;
-  uint32_t sel_here;
-  unsigned long long sel_here_mass;
 };
 
 // A cut of the descending order: tokens with a key above ``key``, and the first ``keep`` (by id) of
@@ -1024,6 +1026,20 @@ __global__ void __launch_bounds__(RT, 2)
   cl.sync();  // (no CTA leaves while another may read its shared memory)
 }
 
+// Shared memory of a slice: a padded vector at either end.
+template <typename T>
+size_t slice_bytes(int vocab, int ctas) {
+  return ((size_t)((vocab + ctas - 1) / ctas) * sizeof(T) + 47) / 16 * 16;
+}
+// The largest slice that leaves room for two CTAs on an SM.
+size_t max_pair_bytes(int dev) {
+  int per_sm = 0, reserved = 0;
+  cudaDeviceGetAttribute(&per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev);
+  cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, dev);
+  const size_t one = (size_t)per_sm / 2;
+  return one > reserved + sizeof(Shared) ? one - reserved - sizeof(Shared) : 0;
+}
+
 template <typename T>
 int launch_sample_rows(const void* logits, int rows, int vocab, long long row_stride, const float* temperature,
                        const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform,
@@ -1031,20 +1047,28 @@ int launch_sample_rows(const void* logits, int rows, int vocab, long long row_st
   int dev = 0, sms = 148, ctas = 1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NE_ERR_CUDA;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // Slices of up to 80 KB, two CTAs an SM: the barriers of a larger cluster cost more than its shorter
-  // slices save (measured, 320 rows of 151,936 bf16, top-k 20: 2 / 4 / 8 CTAs 97 / 79 / 123 us). Few rows
-  // leave SMs idle, and slices above 8,192 tokens are halved then; where every SM has one CTA, above
+  // Slices that two CTAs an SM have room for, as far as clusters of four (fp32: of two) give them, then
+  // slices of up to 80 KB: the barriers of a larger cluster cost more than its shorter slices save (measured, 320
+  // rows of 151,936 bf16, top-k 20: 2 / 4 / 8 CTAs 97 / 79 / 123 us), but half the CTAs an SM cost more than the
+  // next size does: 320 rows of 80,000 bf16 in 2 / 4 CTAs, mixed settings 166 / 142 us, top-k 20 88 / 74, top-p
+  // 221 / 206; 640 of 40,000 in 1 / 2 162 / 148, 91 / 90, 225 / 206; 640 of 20,000 fp32 in 1 / 2 131 / 125,
+  // 86 / 86, 184 / 184. Not so for 320 of 160,000 bf16 in 4 / 8 (279 / 287, 137 / 137, 412 / 438), nor for 40,000
+  // fp32 in 2 / 4, where top-p's selection passes lose more than the rest gains (127 / 119, 82 / 72, 176 / 209).
+  // Few rows leave SMs idle, and slices above 8,192 tokens are halved then; where every SM has one CTA, above
   // 14,000 (measured, rows of mixed settings: slices of 16,000 / 19,000 / 20,000 tokens halved take 60 -> 47,
   // 125 -> 90 and 70 -> 55 us, of 12,500 58 -> 67).
-  while (ctas < MAX_CLUSTER && (size_t)vocab * sizeof(T) > (80u << 10) * ctas) ctas *= 2;
+  const size_t pair_bytes = max_pair_bytes(dev);
+  const int paired = sizeof(T) == 2 ? 4 : 2;
+  while (ctas < MAX_CLUSTER && slice_bytes<T>(vocab, ctas) > (ctas < paired ? pair_bytes : MID_SLICE_BYTES)) ctas *= 2;
   while (ctas < MAX_CLUSTER && (long long)rows * ctas <= sms &&
          vocab > (2LL * rows * ctas <= sms ? 8192 : 14000) * ctas)
     ctas *= 2;
   const int slice = (vocab + ctas - 1) / ctas;
-  const size_t smem = ((size_t)slice * sizeof(T) + 47) / 16 * 16;  // (a padded vector at either end)
+  const size_t smem = slice_bytes<T>(vocab, ctas);
   // rows that do not all start at once are put in order (320 rows of mixed settings 228 -> 176 us; of one
   // setting, where the order gains nothing, 33 -> 41 to 660 -> 670)
-  const int ordered = top_p && (long long)rows * ctas > 2LL * sms && rows <= 4096 ? rows : 0;
+  const int resident = smem <= pair_bytes ? 2 : 1;
+  const int ordered = top_p && (long long)rows * ctas > (long long)resident * sms && rows <= 4096 ? rows : 0;
   if (smem > MAX_SLICE_BYTES) return NE_ERR_UNSUPPORTED;
   static bool done[64] = {};
   if (!done[dev]) {

@@ -283,3 +283,14 @@ def test_no_rows_and_refusals(ops, cuda_device) -> None:
             ops.sample_logits(*args)
     with pytest.raises(submodule("_lib").NativeError):
         ops.sample_logits(torch.zeros(1, 262145, device=cuda_device), u[:1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("edge", [38704, 77408, 163776])
+def test_either_side_of_the_slices_that_two_ctas_hold(ops, cuda_device, edge, dtype) -> None:
+    """Vocabularies at which a row's cluster grows, and rows that start at once on one side only."""
+    vocab = edge if dtype == torch.bfloat16 else edge // 2
+    for v in (vocab - 1, vocab, vocab + 1, vocab + 500):
+        logits, u = language_logits(45, v, v, cuda_device, dtype)
+        _, _, status = check(ops, logits, [SETTINGS[r % len(SETTINGS)] for r in range(45)], u)
+        assert status == 0
