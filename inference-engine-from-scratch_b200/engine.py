@@ -367,35 +367,59 @@ class B200SpeculativeEngine:
             self.draft_model.copy_blocks(dsrc, ddst, dcount)
         return int(count.item())
 
-    def _prefix_group(self, slot: int) -> tuple[int, int]:
-        """(the slot whose first blocks ``slot`` shares, how many): its prefix's holder, or the source
-        its forks go back to."""
+    def _shares(self, slot: int) -> tuple[int, int] | None:
+        """(the slot whose first blocks ``slot`` has, how many): its fork source, or its prefix's holder."""
+        if slot in self._fork_of:
+            return self._fork_of[slot], self._fork_blocks[slot]
         holder = self._prefix_of.get(slot)
-        if holder is not None:
-            return holder, self._shared_count[slot]
-        blocks = 1 << 30
-        while slot in self._fork_of:
-            blocks = min(blocks, self._fork_blocks[slot])
-            slot = self._fork_of[slot]
-        return slot, blocks
+        return None if holder is None else (holder, self._shared_count[slot])
+
+    def _prefix_groups(self, slots: list[int]) -> list[tuple[int, list[int]]]:
+        """(blocks, batch entries) of the groups that read their first blocks together. The entries below one
+        slot of the tree of prefixes and forks share as many of its blocks as the one that shares the
+        fewest; of all such sets the one that saves the most reads, (entries - 1) x blocks, becomes a
+        group, then the next one among the entries that are left."""
+        everything = 1 << 30  # (a slot has all of its own blocks)
+        below: dict[int, list[tuple[int, int]]] = {}  # slot -> (blocks of it, entry) for each entry below it
+        for i, slot in enumerate(slots):
+            blocks = everything
+            while blocks > 0:
+                below.setdefault(slot, []).append((blocks, i))
+                parent = self._shares(slot)
+                if parent is None:
+                    break
+                slot, blocks = parent[0], min(blocks, parent[1])
+        below = {slot: sorted(entries, key=lambda e: -e[0]) for slot, entries in below.items() if len(entries) > 1}
+        grouped: set[int] = set()
+
+        def best(entries: list[tuple[int, int]]) -> tuple[int, int, int]:
+            """(reads saved, blocks, entries) of the best group among the first entries."""
+            return max(((n * blocks, blocks, n + 1) for n, (blocks, _) in enumerate(entries) if blocks < everything),
+                       key=lambda g: g[0], default=(0, 0, 0))
+
+        found = {slot: best(entries) for slot, entries in below.items()}
+        groups = []
+        while found:
+            slot = max(found, key=lambda x: found[x][0])
+            saved, blocks, n = found[slot]
+            if saved == 0:
+                break
+            members = [i for _, i in below[slot][:n]]
+            groups.append((blocks, sorted(members)))
+            grouped.update(members)
+            for other, entries in list(below.items()):
+                left = [e for e in entries if e[1] not in grouped]
+                if len(left) < len(entries):
+                    below[other], found[other] = left, best(left)
+        return groups
 
     def _fill_groups(self, slots: list[int], host: torch.Tensor) -> None:
-        """Entry groups and prefix lengths of a batch: entries with the same root, two at least, share as
-        many blocks as the one among them that shares the fewest."""
-        members: dict[int, list[int]] = {}
-        shared: dict[int, int] = {}
-        for i, s in enumerate(slots):
-            root, blocks = self._prefix_group(s)
-            members.setdefault(root, []).append(i)
-            shared[root] = min(shared.get(root, 1 << 30), blocks)
+        """Entry groups and prefix lengths of a batch."""
         entry_group, prefix_blocks = [-1] * self.max_seqs, [0] * self.max_seqs
-        g = 0
-        for root, entries in members.items():
-            if len(entries) > 1 and 0 < shared[root] < 1 << 30:
-                prefix_blocks[g] = shared[root]
-                for i in entries:
-                    entry_group[i] = g
-                g += 1
+        for g, (blocks, entries) in enumerate(self._prefix_groups(slots)):
+            prefix_blocks[g] = blocks
+            for i in entries:
+                entry_group[i] = g
         host.copy_(torch.tensor([entry_group, prefix_blocks], dtype=torch.int32))
 
     @contextlib.contextmanager

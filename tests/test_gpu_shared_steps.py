@@ -182,6 +182,31 @@ def test_forks_of_a_prefix_itself_keep_it(pkg, make, on) -> None:
     assert eng.state.num_free_blocks() == 192
 
 
+def test_a_short_fork_leaves_the_others_their_prefix(pkg, make) -> None:
+    """One user's fork cut inside the first block, and one in the third: the group on the device holds the others
+    and their whole prefix, and every sequence takes the tokens that it takes without sharing."""
+    prompts = prompts_with_prefix(pkg, 160, 4)
+    outs = {}
+    for on in (False, True):
+        eng = make(shared=on)
+        holder = eng.add_prefix(prompts[0][:160])
+        slots = eng.add_requests(prompts, [30] * 4, ignore_eos=True, prefix=holder)
+        eng.prefill(slots)
+        slots += eng.fork(slots[0], 1, at=5) + eng.fork(slots[0], 1, at=40)
+        out = {s: [] for s in slots}
+        for _ in range(4):
+            for s, t in eng.step(slots).tokens.items():
+                out[s] += t
+        outs[on] = [out[s] for s in slots]
+        if on:
+            entry_group, prefix_blocks = eng._groups_dev.tolist()
+            assert entry_group == [0, 0, 0, 0, -1, -1, -1, -1] and prefix_blocks[:2] == [10, 0]
+        eng.release(slots)
+        eng.drop_prefix(holder)
+        assert eng.state.num_free_blocks() == 192
+    assert outs[True] == outs[False]
+
+
 def test_fork_step_and_sample_by_hand(pkg, make, cuda_device) -> None:
     """A user's own loop: prefill, fork, one step, and next tokens drawn from the step's logits with
     top-k, top-p and min-p; the draw equals the definition on those logits."""
