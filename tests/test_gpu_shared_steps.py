@@ -182,6 +182,90 @@ def test_forks_of_a_prefix_itself_keep_it(pkg, make, on) -> None:
     assert eng.state.num_free_blocks() == 192
 
 
+def steps_of(eng, slots, n):
+    """The tokens of ``n`` steps, and whether they wrote the shared attention's workspace."""
+    eng._groups_ws.zero_()
+    out = {s: [] for s in slots}
+    for _ in range(n):
+        for s, t in eng.step(slots).tokens.items():
+            out[s] += t
+    return [out[s] for s in slots], bool(eng._groups_ws.any())
+
+
+@pytest.mark.parametrize("kv_int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("graphs", [True, False], ids=["graphs", "eager"])
+def test_steps_read_a_groups_prefix_through_its_first_member(pkg, make, kv_int8, graphs) -> None:
+    """Users of a prefix and forks of a loner are the groups on the device, and the steps use them: the blocks
+    that the other members' own tables name at a shared prefix are not read."""
+    prompts = prompts_with_prefix(pkg, 150, 3)
+    lone = pkg.make_prompt(pkg.SMALL_TEST.vocab_size, 70, 9, False)
+    outs = []
+    for moved in (False, True):
+        eng = make(kv_int8, cuda_graphs=graphs)
+        holder = eng.add_prefix(prompts[0][:150])
+        slots = eng.add_requests(prompts, [40] * 3, ignore_eos=True, prefix=holder)
+        slots.append(eng.add_request(lone, 40, ignore_eos=True))
+        eng.prefill(slots)
+        slots += eng.fork(slots[3], 2)
+        eng.step(slots)
+        entry_group, prefix_blocks = eng._groups_dev.tolist()
+        assert entry_group[:6] == [0, 0, 0, 1, 1, 1] and entry_group[6:] == [-1, -1]
+        assert prefix_blocks[:3] == [9, 4, 0]  # (150 and 70 cached tokens)
+        saved = eng.state.block_tables.clone()
+        if moved:
+            other = int(saved[holder, 9])  # (the prefix's last block, partly filled and shared with none)
+            eng.state.block_tables[slots[1], :9] = other
+            eng.state.block_tables[slots[2], 2:5] = other
+            eng.state.block_tables[slots[5], :4] = other
+        tokens, ran = steps_of(eng, slots, 4)
+        assert ran
+        outs.append(tokens)
+        rows = torch.tensor(slots, device=saved.device)
+        eng.state.block_tables[rows, :9] = saved[rows, :9]
+        eng.release(slots)
+        eng.drop_prefix(holder)
+        assert eng.state.num_free_blocks() == 192
+    assert outs[0] == outs[1]
+
+
+def test_a_lone_sequences_steps_leave_the_shared_attention_alone(pkg, make) -> None:
+    eng = make()
+    s = eng.add_request(prompts_with_prefix(pkg, 60, 1)[0], 30, ignore_eos=True)
+    eng.prefill([s])
+    assert not steps_of(eng, [s], 3)[1]
+    eng.release([s])
+
+
+def test_reused_slots_and_forks_show_their_groups(pkg, make) -> None:
+    """Requests, loners and forks in the same two slots, one after the other: the groups on the device follow."""
+    eng = make(max_seqs=3)
+    prompts = prompts_with_prefix(pkg, 200, 2)
+    holder = eng.add_prefix(prompts[0][:200])
+
+    def groups(slots):
+        assert sorted(slots) == [1, 2]
+        eng.step(slots)
+        entry_group, prefix_blocks = eng._groups_dev.tolist()
+        return entry_group[:2], prefix_blocks[0]
+
+    def served(prompts, prefix):
+        slots = eng.add_requests(prompts, [20] * len(prompts), ignore_eos=True, prefix=prefix)
+        eng.prefill(slots)
+        return slots
+
+    for _ in range(2):
+        slots = served(prompts, holder)
+        assert groups(slots) == ([0, 0], 12)
+        eng.release(slots)
+        slots = served([p[100:] for p in prompts], None)
+        assert groups(slots) == ([-1, -1], 0)
+        eng.release(slots)
+        slots = served([prompts[0]], None)
+        slots += eng.fork(slots[0], 1, at=50)
+        assert groups(slots) == ([0, 0], 3)
+        eng.release(slots)
+
+
 def test_a_short_fork_leaves_the_others_their_prefix(pkg, make) -> None:
     """One user's fork cut inside the first block, and one in the third: the group on the device holds the others
     and their whole prefix, and every sequence takes the tokens that it takes without sharing."""
