@@ -107,9 +107,10 @@ __device__ __forceinline__ float max2(float a, float b) {
 // ---------------------------------------------------------------- prefixes: the division of the work
 // A group's vectors of one KV head are cut into items of up to 256: one or two query tiles, which share
 // every tile of 128 keys. A key tile costs an item 3 units of work with one query tile and 4 with two
-// (measured, bf16: 3,000 and 4,000 cycles; int8, bound by the conversion: 6,900 and 7,400). The units of all (group, head, item) in turn are divided
-// evenly over the CTAs: CTA c does the key tiles that start in its ceil(W / CTAs) units from
-// c ceil(W / CTAs) on.
+// (measured, bf16: 3,000 and 4,000 cycles). An int8 pool is divided by the same units although its tiles take
+// 6,900 and 7,400: there a share of single query tiles takes up to a quarter longer than one of pairs. The
+// units of all (group, head, item) in turn are divided evenly over the CTAs: CTA c does the key tiles that
+// start in its ceil(W / CTAs) units from c ceil(W / CTAs) on.
 __device__ __forceinline__ int key_tiles(int blocks) { return (blocks + 7) / 8; }
 __device__ __forceinline__ int item_units(int vec) { return vec > TILE ? 4 : 3; }
 // units of one KV head
@@ -188,7 +189,8 @@ __device__ __forceinline__ void add_prefix(Sums& sums, const Parts& parts, int n
 // One 16-token block (logical index kb) against the tile, as tile_block, but values at masked keys do
 // not reach the sums whatever they are, and an int8 block holds its integers as they are: the K scale
 // (``scales``: lane t token t's, lane 16 + t its V scale) multiplies the scores, the V scale the
-// weights, both in fp32 (one rounding of the weights, none of keys and values).
+// weights, both in fp32. The weights are rounded to bf16 for the product with V (2^-8 of each at most), as
+// tile_block rounds them, since the tensor cores take both operands in V's type; their sum is of the fp32 ones.
 template <bool INT8>
 __device__ __forceinline__ void own_block(TileState& ts, uint32_t k_s, uint32_t v_s, int kb, uint32_t scales,
                                           int lane) {
@@ -335,6 +337,8 @@ static_assert((2 * 4 * 16 * D + 2 * 2 * 4 * 16) * 4 <= 4 * 4 * BLOCK_BYTES, "mer
 // cycles after its start (entry, positions, table). 256 entries of 100 own tokens on average and 8 KV heads,
 // alone and from DRAM: 39 us, 115 MB. Three or four stages a warp, two blocks a softmax step, heads as the
 // fastest grid axis, and CTAs beside prefix_kernel's (which then slows as much) were measured: none is faster.
+// Spills, by ptxas, in the variants of two query tiles alone (128 registers): bf16 64 bytes stored and 56 loaded,
+// int8 144 and 104.
 template <bool INT8, int NW, int NT>
 __global__ void __launch_bounds__(32 * NW * NT, NT == 2 ? 2 : NW == 8 ? 1 : NW == 4 ? 3 : 5)
     own_tokens_kernel(const __nv_bfloat16* __restrict__ q, const void* __restrict__ kc, const void* __restrict__ vc,
@@ -624,7 +628,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // 2^t for two t up to 126 (0 below 2^-127, as the special-function one flushes), on the FMA pipe beside the special-function one:
 // t = n + f, n = rint(t) read off the low bits of t + 1.5 x 2^23, and 2^f on [-1/2, 1/2] by the cubic
-// whose largest relative error is least (7.5e-5; the weight is rounded to bf16, 2^-9, next).
+// whose largest relative error is least (7.5e-5, a fiftieth of the 2^-8 by which the rounding of the weight to
+// bf16 may be off next).
 __device__ __forceinline__ void ex2_poly(uint64_t t2, float& a, float& b) {
   unpack2(t2, a, b);
   t2 = pack2(fmaxf(a, -127.f), fmaxf(b, -127.f));
@@ -725,10 +730,15 @@ __device__ __forceinline__ uint32_t exact_pair(uint32_t word, uint32_t sel) {
 // TMEM), 64 keys a step so that the tensor cores work on one half's products while the other's weights
 // are computed; O is rescaled only when the reference moves by more than 2^8. K and V tiles come through
 // a ring of four slots by 3-D tensor loads of the 16-token pages (int8: loaded and converted by four
-// warps). Bound by the softmax's instructions: 16,384 shared tokens x 1,280 vectors x 8 KV heads (85.9
-// GFLOP) take 103 us, 834 TFLOP/s, with the tensor pipe busy 47% of the time (a pair tile's products alone
-// are 2,048 of its 4,000 cycles); 3 of 8 powers of two run on the FMA pipe. A CTA's
-// fixed costs are about 15,000 cycles: plan 6,000, first query tile 2,700, epilogue 3,500 a segment.
+// warps). P is rounded to bf16 (the tensor cores take P and V in one type; l sums the unrounded weights): 2^-8
+// of a weight at most, as the ordinary attention; int8: after the V scale, keys and values unrounded.
+// Bound by the latency of the softmax's chain, one warp a scheduler and query tile: 16,384 shared tokens x 1,280
+// vectors x 8 KV heads (85.9 GFLOP) take 103 us, 834 TFLOP/s, with the tensor pipe busy 47% of the time (a
+// pair tile's products alone are 2,048 of its 4,000 cycles) and 1.8 of 4 issue slots used; 3 of 8 powers of two
+// run on the FMA pipe. int8: 6,900 cycles a tile, of which a shorter softmax took 2,000 (steps of 32 keys, 9,100
+// before), so that chain counts there too; how much the conversion beside it does was not measured. A CTA's
+// fixed costs are about 15,000 cycles: plan 6,000, first query tile 2,700, epilogue 3,500 a segment. Spills, by
+// ptxas: bf16 28 bytes stored and 44 loaded at 168 registers, int8 80 and 132 at 128.
 template <bool INT8>
 __global__ void __launch_bounds__(pre_threads(INT8), 1)
     prefix_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -918,7 +928,8 @@ __global__ void __launch_bounds__(pre_threads(INT8), 1)
         ok = mbar_wait(&sh.s_full[s][half], (tiles_before + t) & 1u, &sh.abort_flag, status);
         tc_fence_after();
         // int8: 32 keys at a time, the second 32 loaded twice (their maximum, then their weights), for the
-        // scales take registers and what is spilled does not fit what shared memory leaves of the L1
+        // scales take registers and what is spilled does not fit what shared memory leaves of the L1 (64 at
+        // a time spilled inside the step; 9,100 cycles a tile instead of 6,900)
         constexpr int KEYS = INT8 ? HALF / 2 : HALF;
         float x[KEYS];
         tmem_ld32_start(t_s + HALF * half + (INT8 ? KEYS : 0), x);
