@@ -21,7 +21,7 @@
 // their latency (2 of 4 issue slots used), not by the 97 MB: 320 rows of 151,936 bf16 logits, replayed with the
 // logits in L2, take 41 us greedy, 72 to 92 with top-k or min-p, 135 without a filter, 270 with top-p 0.9 at
 // temperature 0.8 and 670 with top-p 0.999 at 1.5 (every third token a candidate), 176 with all of these mixed
-// (188 as a call by itself); one row 14 to 73. With 64 registers, for two CTAs an SM, ptxas spills 180 bytes stored
+// (176 to 188 as calls, by the inputs); one row 14 to 73. With 64 registers, for two CTAs an SM, ptxas spills 180 bytes stored
 // and 392 loaded (bf16; fp32 20 and 80).
 #include <cooperative_groups.h>
 
